@@ -63,7 +63,8 @@ enum {
 /* Bits a kernel sets in a caller's device error word (err_flag). */
 enum {
   XN_DEVERR_RANGE = 1,  /* an id, code or device position outside its table: that part was skipped */
-  XN_DEVERR_WAIT = 2    /* a bounded wait gave up (the rows that block had not finished are NaN) */
+  XN_DEVERR_WAIT = 2,   /* a bounded wait gave up (the rows that block had not finished are NaN) */
+  XN_DEVERR_FULL = 4    /* xn_paged_plan: the step does not fit (pages, table width or token buffer) */
 };
 
 /* Unary ops handled by xn_unary; names follow `enum UnaryOp`
@@ -365,6 +366,127 @@ XN_API int xn_decode_attention_step(void *out, void *k_cache, void *v_cache, con
 
 /* *total_dev += t on the device, ordered on `stream` (end of a decode step). */
 XN_API int xn_position_advance(int64_t *total_dev, int64_t t, void *stream);
+
+/*
+ * Paged KV cache: requests of different lengths served from one pool of pages.
+ *
+ * A layer's pool is k_pages and v_pages, [n_pages, h_kv, page_size, d] as
+ * seen through three strides in elements (page_stride, head_stride,
+ * slot_stride; the d elements of a row are contiguous), the same for both.
+ * page_size is a power of two in [8, 256]. Row i of
+ * block_table [requests, max_blocks] (int32) lists request i's pages in the
+ * order of positions: position p is row p % page_size of page
+ * block_table[i][p / page_size]. A slot names a row of the pool:
+ * page * page_size + p % page_size. Tokens of a step are packed request after
+ * request: request i's are q_start[i] .. q_start[i + 1] - 1. There is no
+ * reference counterpart: the reference's caches (mimi-rs/src/models/mimi.rs:
+ * 1122-1153, pocket_tts/src/transformer.rs:16-33) hold one position for the
+ * whole batch.
+ */
+
+/* Largest number of requests in one step. */
+#define XN_PAGED_MAX_REQUESTS 8192
+
+/*
+ * The bookkeeping of a step, built on the device from request lengths, in one
+ * launch. For request i with lens[i] cached positions, new_len[i] >= 0 more
+ * tokens are planned; new_len[i] < 0 ends the request. Free pages wait in a
+ * ring: ring_state = {head, count}, the count entries of free_ring [n_pages]
+ * from head on (modulo n_pages).
+ *   - Growing requests, in order, take the pages they lack from the ring's
+ *     head into their next block_table entries; ending requests, in order,
+ *     return theirs behind its last entry (they are not taken in this step).
+ *     A page must belong to one request only. Other entries of both arrays
+ *     are left as they were.
+ *   - kv_len[i] = lens[i] + new_len[i] (0 for an ended request);
+ *     q_start [requests + 1] = prefix sums of the new tokens;
+ *     positions[k] and slots[k] (token_cap entries) of every new token, -1
+ *     behind the last one; ring_state_out = the ring after the step.
+ * All or nothing. A step that needs more pages than the ring holds, a table
+ * row beyond max_blocks or more than token_cap tokens sets XN_DEVERR_FULL;
+ * inputs that contradict one another (a negative length, one beyond
+ * max_blocks * page_size, a ring of more than n_pages entries, a page id
+ * outside [0, n_pages)) set XN_DEVERR_RANGE. Either way table and ring stay as
+ * they were, kv_len = lens, ring_state_out = ring_state, q_start is all 0 and
+ * every position and slot is -1, so that the operators below do nothing.
+ * (Page ids are checked where a token's slot needs them: such a token alone
+ * gets slot -1.) kv_len and ring_state_out must not be lens and ring_state.
+ * requests <= XN_PAGED_MAX_REQUESTS.
+ */
+XN_API int xn_paged_plan(int64_t *q_start, int64_t *kv_len, int64_t *positions, int64_t *slots,
+                         int64_t *ring_state_out, int32_t *block_table, int32_t *free_ring, const int64_t *lens,
+                         const int64_t *new_len, const int64_t *ring_state, int64_t requests, int64_t max_blocks,
+                         int64_t n_pages, int64_t page_size, int64_t token_cap, int *err_flag, void *stream);
+
+/*
+ * RoPE and the cache append of a step's tokens, from the packed projection
+ * qkv [n_tokens, h + 2 h_kv, d] (q | k | v):
+ *   q_out [n_tokens, h, d] = rope(q), pool row slots[k] = rope(k) and v,
+ * at positions[k], cos / sin [max_pos, d/2]. Products and sums are f32, with
+ * one rounding to T (xn_kv_append_rope rounds each product, as the reference
+ * does). A token of slot -1 is padding: nothing of it is read or written. A
+ * slot outside the pool or a position outside the tables skips that token and
+ * sets XN_DEVERR_RANGE. Two tokens must not share a slot. d is 32, 64 or 128;
+ * tensors are 16-byte aligned and strides multiples of 16 bytes.
+ */
+XN_API int xn_paged_append_rope(void *q_out, void *k_pages, void *v_pages, const void *qkv, const void *cos,
+                                const void *sin, const int64_t *positions, const int64_t *slots, int64_t n_tokens,
+                                int64_t h, int64_t h_kv, int64_t d, int64_t max_pos, int64_t n_pages,
+                                int64_t page_size, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                                int interleaved, int dtype, int *err_flag, void *stream);
+
+/*
+ * Causal attention of a step's tokens over the pages. Request i's t =
+ * q_start[i + 1] - q_start[i] tokens are its last t positions: token j is at
+ * p = kv_len[i] - t + j and sees keys max(0, p - window + 1) .. p (all of
+ * 0 .. p when window == 0). With scores s = scale * (q . k):
+ *   out [n_tokens, h, d] = sum_k exp(s_k) v_k / sum_k exp(s_k),
+ * query head a reading kv head a / (h / h_kv). Sums and the running maximum
+ * are f32; bf16 / f16 weights exp(s - max) are rounded to T for the product
+ * with v. Keys a token does not see take no part, whatever their rows hold
+ * (stale rows, infinities, NaN); a token that sees none (p < 0) gives zeros. A
+ * page id outside [0, n_pages) reads as rows of zeros and sets
+ * XN_DEVERR_RANGE; a request whose q_start or kv_len lies outside the tensors
+ * is skipped and sets it too. Rows outside all requests are left as they were.
+ *
+ * q rows start every q_tok_stride elements (a slice of a packed projection
+ * will do). max_new is the largest t the caller expects: it chooses the kernel
+ * (results hold for any t). scale is positive and finite; d is 32, 64 or 128;
+ * h is a multiple of h_kv, h / h_kv <= 64; tensors are 16-byte aligned and
+ * strides multiples of 16 bytes. workspace (device, 16-byte aligned) holds at
+ * least xn_paged_attention_workspace() bytes of these sizes; nothing in it
+ * needs to be set, nothing is kept in it between calls, and calls that may run
+ * at the same time (other streams, other graphs) need their own.
+ */
+XN_API int xn_paged_attention(void *out, const void *q, const void *k_pages, const void *v_pages,
+                              const int32_t *block_table, const int64_t *q_start, const int64_t *kv_len,
+                              int64_t n_tokens, int64_t requests, int64_t h, int64_t h_kv, int64_t d,
+                              int64_t n_pages, int64_t page_size, int64_t max_blocks, int64_t q_tok_stride,
+                              int64_t page_stride, int64_t head_stride, int64_t slot_stride, int64_t max_new,
+                              int64_t window, float scale, int dtype, void *workspace, int64_t workspace_bytes,
+                              int *err_flag, void *stream);
+
+/* Writes the workspace size of xn_paged_attention, in bytes, to *bytes (a host pointer). */
+XN_API int xn_paged_attention_workspace(int64_t *bytes, int64_t n_tokens, int64_t requests, int64_t h,
+                                        int64_t h_kv, int64_t d, int64_t max_new, int dtype);
+
+/*
+ * RMSNorm with the residual's addition and an output in 8 bits:
+ *   h = src, or T(src + branch); residual_out = h if not NULL
+ *   y = h / sqrt(sum(h^2)/cols + eps) * alpha[col]             (f32)
+ *   scales[row, g] = max |y| over the g-th `group` columns / 448
+ *   dst = e4m3(y / scale), 0 where the scale is 0
+ * so that dst * scale stands for y. group is 0 (one scale per row, scales
+ * [rows]) or 32, 64 or 128 and a divisor of cols (scales [rows, cols/group]).
+ * dst holds OCP e4m3 bytes (448 the largest value). A NaN among a group's y
+ * makes its scale and all its values NaN; a group whose largest |y| is
+ * infinite gets scale inf, values 0, and NaN where y is infinite.
+ * eps must be > 0; residual_out may alias src or branch. The 8-bit form of
+ * xn_rms_norm for the projections that follow it (llama.rs:306-316).
+ */
+XN_API int xn_rms_norm_q8(void *dst, float *scales, void *residual_out, const void *src, const void *alpha,
+                          const void *branch, int64_t rows, int64_t cols, int64_t group, float eps, int dtype,
+                          void *stream);
 
 /*
  * Row-shard plan for splitting `rows` over `world` GPUs: contiguous blocks of

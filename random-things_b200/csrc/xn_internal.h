@@ -40,6 +40,10 @@ inline int64_t pow2_ceil(int64_t v) {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Checks a paged KV pool's sizes and strides (in elements) for `op`; XN_OK or the error recorded.
+int check_pages(const char *op, int64_t n_pages, int64_t page_size, int64_t h_kv, int64_t d, int64_t page_stride,
+                int64_t head_stride, int64_t slot_stride, int dtype);
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 

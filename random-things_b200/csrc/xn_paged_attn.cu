@@ -1,0 +1,485 @@
+// xn_paged_attn.cu - causal attention of a step's new tokens over a paged KV
+// cache, for sm_100a: the schedule, the f32 kernel, the join of split work.
+//
+//   o = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m),  s_k = scale (q . k),  m = max_k s_k
+//
+// in one pass over the keys: a tile of scores moves the running maximum m,
+// the sums so far shrink by exp(m_old - m_new), and the tile's terms are added.
+#include <math.h>
+
+#include "xn_paged_attn.cuh"
+
+namespace xn {
+namespace paged {
+namespace {
+
+constexpr int kSchedThreads = 1024;
+
+__device__ __forceinline__ int64_t block_scan_excl(int64_t v, int64_t *tot, int64_t &all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) tot[warp] = s;
+  __syncthreads();
+  int64_t before = 0;
+  all = 0;
+  for (int w = 0; w < kSchedThreads / 32; ++w) {
+    const int64_t t = tot[w];
+    if (w < warp) before += t;
+    all += t;
+  }
+  __syncthreads();
+  return before + s - v;
+}
+
+// Builds the work list: one block, since it is a few thousand additions.
+__global__ void __launch_bounds__(kSchedThreads) paged_schedule_kernel(const Args a) {
+  griddep_wait();
+  griddep_release();
+  extern __shared__ int32_t tile_pre[];  // tiles of the requests before request i
+  __shared__ int64_t tot[kSchedThreads / 32];
+  const int n = a.requests, tid = threadIdx.x;
+  int64_t carry = 0, all;
+  int bad = 0;
+  for (int base = 0; base < n; base += kSchedThreads) {
+    const int i = base + tid;
+    int64_t v = 0;
+    if (i < n) {
+      const int64_t q0 = a.q_start[i], q1 = a.q_start[i + 1], kv = a.kv_len[i];
+      if (q0 < 0 || q1 < q0 || q1 > a.n_tokens || kv < 0 || kv > (a.max_blocks << a.page_shift))
+        bad = XN_DEVERR_RANGE;
+      else
+        v = (q1 - q0 + a.tile_tokens - 1) / a.tile_tokens;
+    }
+    const int64_t before = carry + block_scan_excl(v, tot, all);
+    if (i < n) tile_pre[i] = static_cast<int32_t>(before);
+    carry += all;
+  }
+  if (bad && a.err_flag != nullptr) atomicOr(a.err_flag, bad);
+  // Requests with overlapping tokens (q_start not ascending) could list more
+  // tiles than the workspace has room for.
+  int64_t n_tiles = carry;
+  const int64_t room = a.n_tokens / a.tile_tokens + n;
+  if (n_tiles > room) {
+    if (tid == 0 && a.err_flag != nullptr) atomicOr(a.err_flag, XN_DEVERR_RANGE);
+    n_tiles = 0;
+  }
+  __syncthreads();
+  carry = 0;
+  for (int64_t base = 0; base < n_tiles; base += kSchedThreads) {
+    const int64_t e = base + tid;
+    Tile t{};
+    if (e < n_tiles) {
+      int lo = 0, hi = n;  // last request with tile_pre <= e
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tile_pre[mid] <= e)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const int64_t j0 = (e - tile_pre[lo]) * a.tile_tokens, q0 = a.q_start[lo], nt = a.q_start[lo + 1] - q0;
+      t.req = lo;
+      t.tok0 = static_cast<int32_t>(q0 + j0);
+      t.ntok = static_cast<int32_t>(nt - j0 < a.tile_tokens ? nt - j0 : a.tile_tokens);
+      t.pos0 = a.kv_len[lo] - nt + j0;
+      const int64_t end = t.pos0 + t.ntok;  // keys the last row sees end here
+      const int64_t u = end <= 0 ? 1 : (end + a.bn - 1) / a.bn - first_unit(t, a.window, a.bn);
+      t.units = static_cast<int32_t>(u);
+    }
+    t.ustart = carry + block_scan_excl(t.units, tot, all);
+    carry += all;
+    if (e < n_tiles) a.tiles[e] = t;
+  }
+  const int64_t w = carry * a.h_kv;
+  int64_t ctas = (w + a.min_units - 1) / a.min_units;
+  if (ctas > a.parts) ctas = a.parts;
+  if (tid == 0) {
+    a.header->n_tiles = n_tiles;
+    a.header->units = w;
+    a.header->ctas = static_cast<int32_t>(ctas);
+  }
+  // The thread that holds a tile marks the parts that begin in it.
+  for (int64_t e = tid; e < n_tiles; e += kSchedThreads) {
+    const Tile t = a.tiles[e];
+    const int64_t lo = t.ustart * a.h_kv, hi = lo + static_cast<int64_t>(t.units) * a.h_kv;
+    for (int64_t c = (lo * ctas + w - 1) / w; c < ctas; ++c) {
+      const int64_t at = c * w / ctas;
+      if (at >= hi) break;
+      const int64_t r = at - lo;
+      a.starts[c] = Start{static_cast<int32_t>(e), static_cast<int32_t>(r / t.units), static_cast<int32_t>(r % t.units), 0};
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Tiles on the CUDA cores: 16 x 16 threads, each with kRows rows and every
+// 16th key (scores) or a run of columns (output).
+// ---------------------------------------------------------------------------
+template <int D, int BM>
+struct SimtCfg {
+  static constexpr int kBN = 64, kThreads = 256, kRows = BM / 16;
+  static constexpr int kQ = BM * D, kK = kBN * (D + 4), kV = kBN * D, kP = BM * (kBN + 4);
+  static constexpr size_t kSmem = sizeof(float) * (kQ + kK + kV + kP);
+};
+
+template <typename T, int D, int BM>
+__global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
+  griddep_wait();
+  griddep_release();
+  using Cfg = SimtCfg<D, BM>;
+  constexpr int BN = Cfg::kBN, R = Cfg::kRows, V = Elem<T>::kVec, CP = D / 16;
+  extern __shared__ __align__(16) float simt_smem[];
+  float *Qs = simt_smem, *Ks = Qs + Cfg::kQ, *Vs = Ks + Cfg::kK, *Ps = Vs + Cfg::kV;
+  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+  const int part = blockIdx.x;
+  const int64_t page_mask = (int64_t{1} << a.page_shift) - 1;
+  Tile t;
+  for (Walk w(a, part); w.get(a, t); w.next(a)) {
+    const int rows = t.ntok * a.group;
+    __syncthreads();  // the last segment's reads of Qs are done
+    for (int i = tid; i < BM * (D / V); i += 256) {
+      const int row = i / (D / V), c = i % (D / V) * V;
+      float x[V] = {};
+      if (row < rows) {
+        const int64_t tok = t.tok0 + row / a.group, head = w.head * a.group + row % a.group;
+        unpack<T>(ld_cached(static_cast<const T *>(a.q) + tok * a.q_stride + head * D + c), x);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) Qs[row * D + c + j] = x[j];
+    }
+    float o[R][CP], m[R], l[R];
+    int64_t pos[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+      pos[r] = t.pos0 + (ty * R + r) / a.group;
+#pragma unroll
+      for (int c = 0; c < CP; ++c) o[r][c] = 0.f;
+    }
+    const int64_t key_hi = t.pos0 + t.ntok;  // keys from here on are seen by no row
+    const int64_t key_lo = a.window > 0 ? t.pos0 - a.window + 1 : 0;
+    const int64_t u0 = first_unit(t, a.window, BN) + w.k;
+    for (int64_t u = u0; u < u0 + w.take; ++u) {
+      const int64_t key0 = u * BN;
+      __syncthreads();  // the last tile's reads are done
+      for (int i = tid; i < BN * (D / V); i += 256) {
+        const int row = i / (D / V), c = i % (D / V) * V;
+        const int64_t key = key0 + row;
+        float kx[V] = {}, vx[V] = {};
+        if (key < key_hi && key >= key_lo) {
+          const int32_t page = a.table[t.req * a.max_blocks + (key >> a.page_shift)];
+          if (page >= 0 && page < a.n_pages) {
+            const int64_t at = page * a.page_stride + w.head * a.head_stride + (key & page_mask) * a.slot_stride + c;
+            unpack<T>(ld_cached(static_cast<const T *>(a.k) + at), kx);
+            unpack<T>(ld_cached(static_cast<const T *>(a.v) + at), vx);
+          } else if (a.err_flag != nullptr) {
+            atomicOr(a.err_flag, XN_DEVERR_RANGE);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          Ks[row * (D + 4) + c + j] = kx[j];
+          Vs[row * D + c + j] = vx[j];
+        }
+      }
+      __syncthreads();
+      float s[R][4] = {};
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) {
+        float4 kf[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4 *>(&Ks[(tx + 16 * j) * (D + 4) + d]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float4 qf = *reinterpret_cast<const float4 *>(&Qs[(ty * R + r) * D + d]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[r][j] = __fmaf_rn(qf.x, kf[j].x, s[r][j]);
+            s[r][j] = __fmaf_rn(qf.y, kf[j].y, s[r][j]);
+            s[r][j] = __fmaf_rn(qf.z, kf[j].z, s[r][j]);
+            s[r][j] = __fmaf_rn(qf.w, kf[j].w, s[r][j]);
+          }
+        }
+      }
+      // Some row does not see some key: the keys' part in each row is then decided one by one.
+      const bool masked = key0 + BN - 1 > t.pos0 || (a.window > 0 && key0 <= key_hi - 1 - a.window);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        bool seen[4];
+        float mx = m[r];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t key = key0 + tx + 16 * j;
+          seen[j] = !masked || (key <= pos[r] && (a.window == 0 || key > pos[r] - a.window));
+          if (seen[j]) mx = fmaxf(mx, s[r][j]);
+        }
+#pragma unroll
+        for (int b = 8; b > 0; b >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, b));
+        const float base = mx == -INFINITY ? 0.f : mx;
+        const float shrink = ex2_approx((m[r] - base) * a.scale_log2);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = seen[j] ? ex2_approx((s[r][j] - base) * a.scale_log2) : 0.f;
+          sum += p;
+          Ps[(ty * R + r) * (BN + 4) + tx + 16 * j] = seen[j] ? p : -1.f;  // -1: no part in the row
+        }
+#pragma unroll
+        for (int b = 8; b > 0; b >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, b);
+        m[r] = mx;
+        l[r] = __fmaf_rn(l[r], shrink, sum);
+#pragma unroll
+        for (int c = 0; c < CP; ++c) o[r][c] *= shrink;
+      }
+      __syncwarp();  // a row's weights are written and read by one half warp
+      auto weigh = [&](auto with_mask) {
+#pragma unroll 2
+        for (int k = 0; k < BN; ++k) {
+          float vf[CP];
+#pragma unroll
+          for (int c = 0; c < CP; ++c) vf[c] = Vs[k * D + (CP >= 4 ? (c / 4) * 64 + tx * 4 + c % 4 : tx * CP + c)];
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float p = Ps[(ty * R + r) * (BN + 4) + k];
+#pragma unroll
+            for (int c = 0; c < CP; ++c) {
+              const float x = __fmaf_rn(p, vf[c], o[r][c]);
+              o[r][c] = decltype(with_mask)::value && p < 0.f ? o[r][c] : x;
+            }
+          }
+        }
+      };
+      if (masked)
+        weigh(std::true_type{});
+      else
+        weigh(std::false_type{});
+    }
+    const bool whole = w.whole(t);
+    float *part_o = whole ? nullptr : partial_of(a, part, w.first ? 0 : 1, BM, D);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = ty * R + r;
+      if (row >= rows) continue;
+      const float inv = pos[r] < 0 ? 0.f : __fdiv_rn(1.f, l[r]);
+      const int64_t tok = t.tok0 + row / a.group, head = w.head * a.group + row % a.group;
+      T *dst = static_cast<T *>(a.out) + (tok * a.h + head) * D;
+#pragma unroll
+      for (int c = 0; c < CP; ++c) {
+        const int col = CP >= 4 ? (c / 4) * 64 + tx * 4 + c % 4 : tx * CP + c;
+        if (whole)
+          dst[col] = Elem<T>::from_f32(pos[r] < 0 ? 0.f : o[r][c] * inv);
+        else
+          part_o[row * D + col] = o[r][c];
+      }
+      if (!whole && tx == 0) {
+        part_o[BM * D + row] = m[r];
+        part_o[BM * D + BM + row] = l[r];
+      }
+    }
+  }
+}
+
+// Adds the partial sums of the (tile, head) pairs that were cut, pieces in key
+// order. Block (c, y): the pair cut first at the start of part c + 1, rows from y on.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) paged_combine_kernel(const Args a, int bm) {
+  griddep_wait();
+  griddep_release();
+  const int c = blockIdx.x + 1, ctas = a.header->ctas;
+  if (c >= ctas) return;
+  const Start s = a.starts[c], b = a.starts[c - 1];
+  if (s.k == 0) return;  // nothing is cut here
+  const bool same = b.tile == s.tile && b.head == s.head;
+  if (same && b.k > 0) return;  // cut before: an earlier block's
+  int last = c;                 // the last part with a piece of the pair
+  while (last + 1 < ctas) {
+    const Start n = a.starts[last + 1];
+    if (n.tile != s.tile || n.head != s.head || n.k == 0) break;
+    ++last;
+  }
+  const Tile t = a.tiles[s.tile];
+  constexpr int C = D / 4, RB = 128 / C;  // threads of a row, rows of a block
+  const int col = threadIdx.x % C * 4;
+  for (int row = blockIdx.y * RB + threadIdx.x / C; row < t.ntok * a.group; row += gridDim.y * RB) {
+    float mx = -INFINITY;
+    for (int i = c - 1; i <= last; ++i) {
+      const float *p = partial_of(a, i, i == c - 1 && !same ? 1 : 0, bm, D);
+      mx = fmaxf(mx, p[bm * D + row]);
+    }
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    for (int i = c - 1; i <= last; ++i) {
+      const float *p = partial_of(a, i, i == c - 1 && !same ? 1 : 0, bm, D);
+      const float m = p[bm * D + row];
+      const float f = m == -INFINITY ? 0.f : ex2_approx((m - mx) * a.scale_log2);
+      const float4 x = *reinterpret_cast<const float4 *>(&p[row * D + col]);
+      l = __fmaf_rn(p[bm * D + bm + row], f, l);
+      o.x = __fmaf_rn(x.x, f, o.x);
+      o.y = __fmaf_rn(x.y, f, o.y);
+      o.z = __fmaf_rn(x.z, f, o.z);
+      o.w = __fmaf_rn(x.w, f, o.w);
+    }
+    const int64_t pos = t.pos0 + row / a.group;
+    const float inv = __fdiv_rn(1.f, l);
+    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    const int64_t tok = t.tok0 + row / a.group, head = s.head * a.group + row % a.group;
+    T *dst = static_cast<T *>(a.out) + (tok * a.h + head) * D + col;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dst[j] = Elem<T>::from_f32(pos < 0 ? 0.f : y[j]);
+  }
+}
+
+// How a call is cut: rows of a query tile, keys of a key tile, parts.
+struct Shape {
+  int bm, bn, parts, min_units;
+};
+
+Shape shape_of(int64_t group, int64_t max_new, int dtype) {
+  (void)dtype;
+  const bool few = max_new * group <= 16 && group <= 16;
+  return Shape{few ? 16 : 64, 64, 2 * sm_count(), 4};
+}
+
+struct Layout {
+  int64_t tiles, starts, partial, bytes;
+};
+
+Layout layout_of(const Shape &s, int64_t n_tokens, int64_t requests, int64_t group, int64_t d) {
+  auto up = [](int64_t v) { return (v + 255) & ~int64_t{255}; };
+  Layout l;
+  l.tiles = up(sizeof(Header));
+  const int64_t tt = s.bm / group;
+  l.starts = l.tiles + up(static_cast<int64_t>(sizeof(Tile)) * (n_tokens / tt + requests));
+  l.partial = l.starts + up(static_cast<int64_t>(sizeof(Start)) * (s.parts + 1));
+  l.bytes = l.partial + up(static_cast<int64_t>(sizeof(float)) * 2 * s.parts * s.bm * (d + 2));
+  return l;
+}
+
+template <typename T, int D, int BM>
+void launch_simt(const Args &a, cudaStream_t st) {
+  constexpr size_t smem = SimtCfg<D, BM>::kSmem;
+  cudaFuncSetAttribute(paged_attn_simt_kernel<T, D, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  launch_k(paged_attn_simt_kernel<T, D, BM>, dim3(a.parts), dim3(256), smem, st, a);
+}
+
+template <typename T, int D>
+int launch_attn(const Args &a, const Shape &s, cudaStream_t st, const char *op) {
+  const size_t smem = sizeof(int32_t) * (static_cast<size_t>(a.requests) + 1);
+  launch_k(paged_schedule_kernel, dim3(1), dim3(kSchedThreads), smem, st, a);
+  if (s.bm == 16)
+    launch_simt<T, D, 16>(a, st);
+  else
+    launch_simt<T, D, 64>(a, st);
+  if (a.parts > 1) launch_k(paged_combine_kernel<T, D>, dim3(a.parts - 1, ceil_div(s.bm, 16)), dim3(128), 0, st, a, s.bm);
+  return check_launch(op);
+}
+
+int check_sizes(const char *op, int64_t n_tokens, int64_t requests, int64_t h, int64_t h_kv, int64_t d,
+                int64_t max_new, int dtype) {
+  if (!is_float_dtype(dtype)) return fail(XN_E_DTYPE, "%s: unsupported dtype %d", op, dtype);
+  if (n_tokens < 0 || requests < 0 || max_new < 0) return fail(XN_E_INVALID, "%s: negative size", op);
+  if (h <= 0 || h_kv <= 0 || h % h_kv != 0 || h / h_kv > 64 || h > 65536)
+    return fail(XN_E_INVALID, "%s: h=%lld is not 1 to 64 times h_kv=%lld", op, (long long)h, (long long)h_kv);
+  if (d != 32 && d != 64 && d != 128) return fail(XN_E_INVALID, "%s: head dim %lld not in {32, 64, 128}", op, (long long)d);
+  if (requests > XN_PAGED_MAX_REQUESTS)
+    return fail(XN_E_INVALID, "%s: %lld requests exceed %d", op, (long long)requests, XN_PAGED_MAX_REQUESTS);
+  if (n_tokens > 0x7fffffffLL) return fail(XN_E_INVALID, "%s: too many tokens (%lld)", op, (long long)n_tokens);
+  return XN_OK;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace xn
+
+extern "C" {
+
+int xn_paged_attention_workspace(int64_t *bytes, int64_t n_tokens, int64_t requests, int64_t h, int64_t h_kv,
+                                 int64_t d, int64_t max_new, int dtype) {
+  using namespace xn;
+  const char *op = "xn_paged_attention_workspace";
+  if (bytes == nullptr) return fail(XN_E_INVALID, "%s: null output pointer", op);
+  if (const int rc = paged::check_sizes(op, n_tokens, requests, h, h_kv, d, max_new, dtype)) return rc;
+  const paged::Shape s = paged::shape_of(h / h_kv, max_new, dtype);
+  *bytes = paged::layout_of(s, n_tokens, requests, h / h_kv, d).bytes;
+  return ok();
+}
+
+int xn_paged_attention(void *out, const void *q, const void *k_pages, const void *v_pages, const int32_t *block_table,
+                       const int64_t *q_start, const int64_t *kv_len, int64_t n_tokens, int64_t requests, int64_t h,
+                       int64_t h_kv, int64_t d, int64_t n_pages, int64_t page_size, int64_t max_blocks,
+                       int64_t q_tok_stride, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                       int64_t max_new, int64_t window, float scale, int dtype, void *workspace,
+                       int64_t workspace_bytes, int *err_flag, void *stream) {
+  using namespace xn;
+  const char *op = "xn_paged_attention";
+  if (const int rc = paged::check_sizes(op, n_tokens, requests, h, h_kv, d, max_new, dtype)) return rc;
+  if (const int rc = check_pages(op, n_pages, page_size, h_kv, d, page_stride, head_stride, slot_stride, dtype)) return rc;
+  if (max_blocks < 0 || max_blocks > ((int64_t{1} << 31) - 1024) / page_size)
+    return fail(XN_E_INVALID, "%s: max_blocks=%lld out of range", op, (long long)max_blocks);
+  if (window < 0) return fail(XN_E_INVALID, "%s: negative window", op);
+  if (!(scale > 0.f) || isinf(scale)) return fail(XN_E_INVALID, "%s: scale must be positive and finite", op);
+  if (q_tok_stride < h * d || q_tok_stride % (16 / dtype_bytes(dtype)) != 0)
+    return fail(XN_E_INVALID, "%s: q rows need a stride of at least h * d elements, a multiple of 16 bytes (got %lld)", op,
+                (long long)q_tok_stride);
+  if (n_tokens == 0 || requests == 0) return ok();
+  if (out == nullptr || q == nullptr || k_pages == nullptr || v_pages == nullptr || q_start == nullptr ||
+      kv_len == nullptr || workspace == nullptr || (max_blocks > 0 && block_table == nullptr))
+    return fail(XN_E_INVALID, "%s: null pointer", op);
+  const void *ptrs[] = {out, q, k_pages, v_pages, workspace};
+  for (const void *ptr : ptrs)
+    if (!is_aligned16(ptr)) return fail(XN_E_INVALID, "%s: tensors must be 16-byte aligned", op);
+  const int64_t group = h / h_kv;
+  const paged::Shape s = paged::shape_of(group, max_new, dtype);
+  const paged::Layout l = paged::layout_of(s, n_tokens, requests, group, d);
+  if (workspace_bytes < l.bytes)
+    return fail(XN_E_INVALID, "%s: workspace of %lld bytes, %lld needed", op, (long long)workspace_bytes, (long long)l.bytes);
+  int shift = 0;
+  while ((int64_t{1} << shift) < page_size) ++shift;
+  char *ws = static_cast<char *>(workspace);
+  paged::Args a{};
+  a.out = out;
+  a.q = q;
+  a.k = k_pages;
+  a.v = v_pages;
+  a.table = block_table;
+  a.q_start = q_start;
+  a.kv_len = kv_len;
+  a.n_tokens = n_tokens;
+  a.n_pages = n_pages;
+  a.max_blocks = max_blocks;
+  a.q_stride = q_tok_stride;
+  a.page_stride = page_stride;
+  a.head_stride = head_stride;
+  a.slot_stride = slot_stride;
+  a.window = window;
+  a.requests = static_cast<int32_t>(requests);
+  a.h = static_cast<int32_t>(h);
+  a.h_kv = static_cast<int32_t>(h_kv);
+  a.group = static_cast<int32_t>(group);
+  a.page_shift = shift;
+  a.tile_tokens = static_cast<int32_t>(s.bm / group);
+  a.bn = s.bn;
+  a.parts = s.parts;
+  a.min_units = s.min_units;
+  a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  a.err_flag = err_flag;
+  a.header = reinterpret_cast<paged::Header *>(ws);
+  a.tiles = reinterpret_cast<paged::Tile *>(ws + l.tiles);
+  a.starts = reinterpret_cast<paged::Start *>(ws + l.starts);
+  a.partial = reinterpret_cast<float *>(ws + l.partial);
+  cudaStream_t st = as_stream(stream);
+  XN_DISPATCH_FLOAT(dtype, {
+    if (d == 32) return paged::launch_attn<T, 32>(a, s, st, op);
+    if (d == 64) return paged::launch_attn<T, 64>(a, s, st, op);
+    return paged::launch_attn<T, 128>(a, s, st, op);
+  });
+  return fail(XN_E_DTYPE, "%s: unsupported dtype %d", op, dtype);
+}
+
+}  // extern "C"

@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes
 from pathlib import Path
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -27,7 +27,8 @@ XN_UNARY_SILU, XN_UNARY_GELU_ERF = 0, 1
 XN_LAYOUT_BHTD, XN_LAYOUT_BTHD = 0, 1
 XN_RVQ_MAX_CODEBOOKS = 32
 XN_MASK_RELATIVE, XN_MASK_ABSOLUTE, XN_MASK_CACHE_LEN = 0, 1, 2
-XN_DEVERR_RANGE, XN_DEVERR_WAIT = 1, 2
+XN_DEVERR_RANGE, XN_DEVERR_WAIT, XN_DEVERR_FULL = 1, 2, 4
+XN_PAGED_MAX_REQUESTS = 8192
 MASK_MODES = {"relative": XN_MASK_RELATIVE, "absolute": XN_MASK_ABSOLUTE, "cache_len": XN_MASK_CACHE_LEN}
 
 # Same codes as `enum DType` (mimi-rs/src/dtype.rs:4-10).
@@ -81,6 +82,11 @@ SIGNATURES = {
     "xn_position_advance": [_vp, _i64, _vp],
     "xn_decode_attention_step": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64,
                                  _i64, _int, _f32, _int, _int, _vp, _vp],
+    "xn_paged_plan": [_vp] * 10 + [_i64] * 5 + [_vp, _vp],
+    "xn_paged_append_rope": [_vp] * 8 + [_i64] * 10 + [_int, _int, _vp, _vp],
+    "xn_paged_attention": [_vp] * 7 + [_i64] * 14 + [_f32, _int, _vp, _i64, _vp, _vp],
+    "xn_paged_attention_workspace": [ctypes.POINTER(_i64)] + [_i64] * 6 + [_int],
+    "xn_rms_norm_q8": [_vp] * 6 + [_i64] * 3 + [_f32, _int, _vp],
 }
 _RESTYPE = {"xn_last_error": ctypes.c_char_p}
 
@@ -775,6 +781,232 @@ def position_advance(total_dev: torch.Tensor, t: int) -> None:
     """total_dev += t on the device (the end of a captured decode step)."""
     _total_args(None, total_dev, "position_advance")
     _call("xn_position_advance", _p(total_dev), int(t), _stream(total_dev))
+
+
+# ---------------------------------------------------------------------------
+# Paged KV cache: requests of different lengths on one pool of pages (no
+# reference counterpart; the reference's caches hold one position per batch)
+# ---------------------------------------------------------------------------
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    # The launch goes to the tensors' device, which need not be the current one.
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        _call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            _call(name, *args)
+
+
+def _ints(op: str, dtype: torch.dtype, **ts: torch.Tensor) -> None:
+    for name, t in ts.items():
+        if t.dtype != dtype:
+            raise XnError(f"{op}: {name} must be {dtype}, got {t.dtype}", XN_E_DTYPE)
+
+
+def _err_word(op: str, err_flag: torch.Tensor | None) -> None:
+    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() < 1):
+        raise XnError(f"{op}: err_flag must be an int32 CUDA tensor")
+
+
+def _pool(op: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int, int, int, int]:
+    """(n_pages, h_kv, page_size, d, page stride, head stride, slot stride) of a pool seen as
+    [n_pages, h_kv, page_size, d]; a pool laid out otherwise is passed as a permuted view."""
+    _check_same_shape(k_pages.shape, v_pages.shape, f"{op} pools")
+    if k_pages.dim() != 4:
+        raise XnError(f"{op}: pools must be [n_pages, h_kv, page_size, d], got {tuple(k_pages.shape)}")
+    if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+        raise XnError(f"{op}: pools must share their strides and have a unit last stride")
+    return (*k_pages.shape, *k_pages.stride()[:3])
+
+
+def _on_device(ref: torch.Tensor, op: str, *ts: torch.Tensor | None) -> None:
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.device != ref.device):
+            raise XnError(f"{op}: tensors must be on one CUDA device")
+
+
+class PagedPlan(NamedTuple):
+    """A step's bookkeeping (paged_plan): where each request's tokens begin, the
+    lengths after the step, each token's position and slot (-1: padding), and
+    the free ring's (head, count)."""
+
+    q_start: torch.Tensor
+    kv_len: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    ring_state: torch.Tensor
+
+
+def paged_plan(lens: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_ring: torch.Tensor,
+               ring_state: torch.Tensor, page_size: int, token_cap: int, *, out: PagedPlan | None = None,
+               err_flag: torch.Tensor | None = None) -> PagedPlan:
+    """Plans a step of requests with lens [R] cached positions and new_len [R]
+    more tokens (int64; negative: the request ends and its pages return).
+    Growing requests take the pages they lack from the ring free_ring
+    [n_pages] (int32; ring_state = int64 (head, count)); block_table [R, blocks]
+    (int32) and free_ring are updated in place, the rest comes out in new
+    tensors, or in `out` (which must not be the inputs). A step that does not
+    fit changes nothing, sets XN_DEVERR_FULL in err_flag and gives an empty
+    plan (q_start 0, slots -1); contradictory inputs set XN_DEVERR_RANGE.
+    No host synchronisation: a captured graph may hold the call."""
+    op = "paged_plan"
+    if lens.dim() != 1 or block_table.dim() != 2 or free_ring.dim() != 1:
+        raise XnError(f"{op}: expected lens [R], block_table [R, blocks], free_ring [n_pages]")
+    n, blocks = block_table.shape
+    _check_same_shape(lens.shape, (n,), f"{op} lens")
+    _check_same_shape(new_len.shape, (n,), f"{op} new_len")
+    _check_same_shape(ring_state.shape, (2,), f"{op} ring_state")
+    if token_cap < 0:
+        raise XnError(f"{op}: negative token_cap")
+    dev = _dev(lens, new_len, block_table, free_ring, ring_state, err_flag)
+    if out is None:
+        # One buffer for all five: small calls are bound by their launches.
+        buf = torch.empty(2 * n + 1 + 2 * token_cap + 2, dtype=torch.int64, device=dev)
+        out = PagedPlan(*buf.split([n + 1, n, token_cap, token_cap, 2]))
+    for t, shape in zip(out, ((n + 1,), (n,), (token_cap,), (token_cap,), (2,))):
+        _check_same_shape(t.shape, shape, f"{op} out")
+    _dev(lens, *out)
+    _ints(op, torch.int64, lens=lens, new_len=new_len, ring_state=ring_state)
+    _ints(op, torch.int64, **out._asdict())
+    _ints(op, torch.int32, block_table=block_table, free_ring=free_ring)
+    _err_word(op, err_flag)
+    _call_on(dev, "xn_paged_plan", _p(out.q_start), _p(out.kv_len), _p(out.positions), _p(out.slots),
+             _p(out.ring_state), _p(block_table), _p(free_ring), _p(lens), _p(new_len), _p(ring_state), n, blocks,
+             free_ring.numel(), int(page_size), int(token_cap), _p(err_flag), _stream(lens))
+    return out
+
+
+def paged_append_rope(qkv: torch.Tensor, heads: int, kv_heads: int, cos: torch.Tensor, sin: torch.Tensor,
+                      k_pages: torch.Tensor, v_pages: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, *,
+                      interleaved: bool = True, err_flag: torch.Tensor | None = None,
+                      q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """RoPE on q and k of the packed projection qkv [N, (heads + 2 * kv_heads) * D] at
+    positions [N], k and v written to slots [N] (paged_plan) of the pools
+    [n_pages, kv_heads, page_size, D], q returned as [N, heads, D]. A token of
+    slot -1 is padding: its q row and the pools are left as they were. Unlike
+    kv_append_rope, which repeats the reference's rounding of every product,
+    the rotation is f32 with one rounding."""
+    op = "paged_append_rope"
+    n_pages, hk, page, d, ps, hs, ss = _pool(op, k_pages, v_pages)
+    n = positions.numel()
+    if hk != kv_heads or qkv.numel() != n * (heads + 2 * kv_heads) * d or qkv.shape[0] != n:
+        raise XnError(f"{op}: expected qkv [{n}, ({heads} + 2 * {kv_heads}) * {d}] and {kv_heads} kv heads in the pools, "
+                      f"got {tuple(qkv.shape)} and {hk}")
+    _check_same_shape(slots.shape, positions.shape, f"{op} slots")
+    _check_same_shape(cos.shape, sin.shape, f"{op} cos/sin")
+    if cos.dim() != 2 or cos.shape[1] * 2 != d:
+        raise XnError(f"{op}: cos/sin must be [max_pos, {d // 2}], got {tuple(cos.shape)}")
+    if q_out is None:
+        q_out = torch.empty((n, heads, d), dtype=qkv.dtype, device=qkv.device)
+    else:
+        _check_same_shape(q_out.shape, (n, heads, d), f"{op} q_out")
+    dev = _dev(qkv, cos, sin, positions, slots, q_out, err_flag)
+    _on_device(qkv, op, k_pages, v_pages)
+    _same_dtype(qkv, cos, sin, k_pages, v_pages, q_out)
+    _ints(op, torch.int64, positions=positions, slots=slots)
+    _err_word(op, err_flag)
+    _call_on(dev, "xn_paged_append_rope", _p(q_out), _p(k_pages), _p(v_pages), _p(qkv), _p(cos), _p(sin), _p(positions),
+             _p(slots), n, heads, kv_heads, d, cos.shape[0], n_pages, page, ps, hs, ss, int(interleaved),
+             _dtype_code(qkv), _p(err_flag), _stream(qkv))
+    return q_out
+
+
+def paged_attention_workspace(n_tokens: int, requests: int, heads: int, kv_heads: int, head_dim: int, max_new: int,
+                              dtype: torch.dtype, device) -> torch.Tensor:
+    """A workspace for paged_attention calls of these sizes (bytes). It holds
+    nothing between calls; calls that may run at the same time (streams,
+    graphs) need one each."""
+    if dtype not in FLOAT_DTYPES:
+        raise XnError(f"unsupported dtype {dtype}", XN_E_DTYPE)
+    n = ctypes.c_int64()
+    _call("xn_paged_attention_workspace", ctypes.byref(n), n_tokens, requests, heads, kv_heads, head_dim, max_new,
+          DTYPE_CODES[dtype])
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    q_start: torch.Tensor, kv_len: torch.Tensor, scale: float, *, max_new: int, window: int = 0,
+                    workspace: torch.Tensor | None = None, err_flag: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of q [N, H, D] (rows may be strided: a slice of a packed
+    projection) over the pools [n_pages, Hkv, page_size, D]: request i's tokens
+    q_start[i] .. q_start[i + 1] - 1 are its last positions before kv_len[i],
+    each sees the keys up to its own position, at most the last `window` of
+    them (0: all). H is a multiple of Hkv. Returns [N, H * D] (the out_proj
+    input); rows outside all requests are left as they were, a token at a
+    negative position gives zeros. max_new is the largest number of new tokens
+    of a request that the caller expects; it decides the kernel, not the
+    result. Pages outside the pool read as zeros and set XN_DEVERR_RANGE."""
+    op = "paged_attention"
+    n_pages, hk, page, d, ps, hs, ss = _pool(op, k_pages, v_pages)
+    if q.dim() != 3 or q.shape[2] != d or hk == 0 or q.shape[1] % hk:
+        raise XnError(f"{op}: q must be [N, H, {d}] with H a multiple of {hk}, got {tuple(q.shape)}")
+    n, h, _ = q.shape
+    if n > 0 and (q.stride(2) != 1 or (h > 1 and q.stride(1) != d)):
+        raise XnError(f"{op}: the rows of q must be contiguous")
+    if block_table.dim() != 2:
+        raise XnError(f"{op}: block_table must be [R, blocks], got {tuple(block_table.shape)}")
+    r, blocks = block_table.shape
+    _check_same_shape(kv_len.shape, (r,), f"{op} kv_len")
+    _check_same_shape(q_start.shape, (r + 1,), f"{op} q_start")
+    if out is None:
+        out = torch.empty((n, h * d), dtype=q.dtype, device=q.device)
+    elif out.numel() != n * h * d:
+        raise XnError(f"{op}: out must hold [N, H * D]")
+    if workspace is None:
+        workspace = paged_attention_workspace(n, r, h, hk, d, max_new, q.dtype, q.device)
+    dev = _dev(out, block_table, q_start, kv_len, workspace, err_flag)
+    _on_device(out, op, q, k_pages, v_pages)
+    _same_dtype(q, k_pages, v_pages, out)
+    _ints(op, torch.int64, q_start=q_start, kv_len=kv_len)
+    _ints(op, torch.int32, block_table=block_table)
+    _err_word(op, err_flag)
+    _call_on(dev, "xn_paged_attention", _p(out), _p(q), _p(k_pages), _p(v_pages), _p(block_table), _p(q_start),
+             _p(kv_len), n, r, h, hk, d, n_pages, page, blocks, q.stride(0) if n > 1 else h * d, ps, hs, ss,
+             int(max_new), int(window), float(scale), _dtype_code(q), _p(workspace),
+             workspace.numel() * workspace.element_size(), _p(err_flag), _stream(out))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# RMSNorm with an output in 8 bits
+# ---------------------------------------------------------------------------
+
+def rms_norm_q8(x: torch.Tensor, alpha: torch.Tensor, eps: float, *, branch: torch.Tensor | None = None,
+                group: int = 0, out: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                residual_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """h = x [+ branch]; y = rms_norm(h) with an 8-bit output: returns (q, scales, h)
+    with q (float8_e4m3fn) * scales standing for y, one scale per row (group 0:
+    scales [rows]) or per `group` = 32, 64 or 128 columns (scales
+    [rows, cols / group]). h is x itself without a branch; otherwise it is
+    written to residual_out (which may be x or branch) or a new tensor."""
+    op = "rms_norm_q8"
+    if eps <= 0.0:
+        raise XnError(f"{op} eps must be positive")
+    rows, cols = _rows_cols(x)
+    if group not in (0, 32, 64, 128) or (group and cols % group):
+        raise XnError(f"{op}: group {group} is not 0, 32, 64 or 128 and a divisor of {cols}")
+    _check_same_shape(alpha.shape, (cols,), f"{op} alpha")
+    if branch is not None:
+        _check_same_shape(branch.shape, x.shape, f"{op} branch")
+        if residual_out is None:
+            residual_out = torch.empty_like(x)
+    if residual_out is not None:
+        _check_same_shape(residual_out.shape, x.shape, f"{op} residual_out")
+    shape = (*x.shape[:-1], cols // group) if group else x.shape[:-1]
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    if scales is None:
+        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+    _check_same_shape(out.shape, x.shape, f"{op} out")
+    _check_same_shape(scales.shape, shape, f"{op} scales")
+    dev = _dev(x, alpha, branch, out, scales, residual_out)
+    _same_dtype(x, alpha, branch, residual_out)
+    if out.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise XnError(f"{op}: out must be float8_e4m3fn and scales float32", XN_E_DTYPE)
+    _call_on(dev, "xn_rms_norm_q8", _p(out), _p(scales), _p(residual_out), _p(x), _p(alpha), _p(branch), rows, cols,
+             int(group), float(eps), _dtype_code(x), _stream(x))
+    return out, scales, x if residual_out is None else residual_out
 
 
 # ---------------------------------------------------------------------------
