@@ -7,7 +7,7 @@
 // the sums so far shrink by exp(m_old - m_new), and the tile's terms are added.
 #include <math.h>
 
-#include "xn_paged_attn.cuh"
+#include "xn_paged_attn_tc.h"
 
 namespace xn {
 namespace paged {
@@ -341,8 +341,8 @@ struct Shape {
 };
 
 Shape shape_of(int64_t group, int64_t max_new, int dtype) {
-  (void)dtype;
   const bool few = max_new * group <= 16 && group <= 16;
+  if (!few && dtype != XN_F32) return Shape{kTcRows, kTcKeys, sm_count(), 2};
   return Shape{few ? 16 : 64, 64, 2 * sm_count(), 4};
 }
 
@@ -372,10 +372,13 @@ template <typename T, int D>
 int launch_attn(const Args &a, const Shape &s, cudaStream_t st, const char *op) {
   const size_t smem = sizeof(int32_t) * (static_cast<size_t>(a.requests) + 1);
   launch_k(paged_schedule_kernel, dim3(1), dim3(kSchedThreads), smem, st, a);
-  if (s.bm == 16)
+  if (s.bm == kTcRows) {
+    if (const int rc = launch_tc(a, D, std::is_same_v<T, float> ? XN_F32 : std::is_same_v<T, __half> ? XN_F16 : XN_BF16, st, op)) return rc;
+  } else if (s.bm == 16) {
     launch_simt<T, D, 16>(a, st);
-  else
+  } else if constexpr (std::is_same_v<T, float>) {
     launch_simt<T, D, 64>(a, st);
+  }
   if (a.parts > 1) launch_k(paged_combine_kernel<T, D>, dim3(a.parts - 1, ceil_div(s.bm, 16)), dim3(128), 0, st, a, s.bm);
   return check_launch(op);
 }

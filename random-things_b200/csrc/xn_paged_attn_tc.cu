@@ -1,0 +1,618 @@
+// xn_paged_attn_tc.cu - the paged attention's kernel for chunks of 16-bit
+// tokens on the 5th-generation tensor cores (sm_100a).
+//
+// A CTA takes 256 rows (token, query head of the group) of one kv head: two
+// halves of 128, each with its own softmax warpgroup, scores S and output O in
+// tensor memory. Per key tile of 128 keys:
+//   S = Q K^T      tcgen05.mma, both operands in shared memory
+//   P = exp2(S c - m c), row maxima and sums   one thread a row: no shuffles
+//   O = O + P V    tcgen05.mma, P in tensor memory (over S), V in shared memory
+// While one half's softmax runs, the tensor cores work for the other half.
+// One warp loads: K and V tiles come by TMA, a box per page, swizzled as the
+// MMA reads them, through a ring of stages; another warp issues the MMAs.
+//
+// O stays in tensor memory for all key tiles. When a row's maximum grows by
+// more than 2^8 (in the exponent's units: 8), its warp rescales O; below that
+// the old maximum stays in use, which changes nothing but the common factor
+// of numerator and denominator.
+//
+// Masks. Scores of unseen keys become -inf, weight 0. A weight of 0 does not
+// silence an infinite or NaN value in the product, so in a tile with a mask
+// the V rows that no row sees (beyond the last token, before the window, stale
+// page rows) are zeroed in shared memory, and when a row that some tokens see
+// and others do not holds a non-finite value, the half adds the tile's product
+// on the CUDA cores, each token over its own keys (poisoned tile).
+//
+// Every wait has a time limit; see wait().
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "xn_paged_attn.cuh"
+#include "xn_paged_attn_tc.h"
+
+namespace xn {
+namespace paged {
+namespace {
+
+constexpr int kBM = kTcRows, kBN = kTcKeys, kThreads = 384;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr uint64_t kWaitNs = 2000000000ull;  // a wait gives up after 2 s
+
+template <int D>
+struct TcCfg {
+  static constexpr int kRowBytes = D >= 64 ? 128 : 64;    // bytes of a swizzled row
+  static constexpr int kHalves = D >= 64 ? D / 64 : 1;    // sub-tiles of kRowBytes a row
+  static constexpr int kSub = 128 * kRowBytes;            // bytes of one sub-tile of 128 rows
+  static constexpr int kTile = kHalves * kSub;            // a Q half, a K tile or a V tile
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr size_t kSmem = 1024 + 2 * kTile + kStages * kTile;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Waits for the phase of `parity`; false when it did not come within kWaitNs or
+// another role gave up (then nothing that the phase stands for may be used).
+// Inlined: with a call in the kernel its register split would not take effect.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
+  uint64_t t0 = 0, t;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try(bar, parity)) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t0 == 0) t0 = t;
+    if (*gave_up || t - t0 > kWaitNs) break;
+  }
+  *gave_up = 1;
+  return false;
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes (one lane a row) from / to tensor memory.
+__device__ __forceinline__ void tc_ld32(uint32_t addr, float *r) {
+  uint32_t *u = reinterpret_cast<uint32_t *>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_ld4(uint32_t addr, uint32_t (&u)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t *u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
+      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
+      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+      : "memory");
+}
+
+// D (tensor memory) = A B (+ D): A and B in shared memory, or A in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int row, int head,
+                                         int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          dst),
+      "l"(map), "r"(bar), "r"(x), "r"(row), "r"(head), "r"(page)
+      : "memory");
+}
+
+// Shared-memory operand descriptor. Low word: address and leading byte offset
+// in 16-byte units (so a step of n bytes adds n / 16; addresses stay below
+// 2^18); high word: stride byte offset, version 1, swizzle of 128 (code 2) or
+// 64 bytes (code 4).
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return addr >> 4 | (lbo >> 4) << 16; }
+constexpr uint32_t desc_hi(uint32_t sbo, uint32_t swizzle) { return sbo >> 4 | 1u << 14 | swizzle << 29; }
+
+// Byte offset of 16-byte chunk j of row r in a swizzled tile.
+template <int D>
+__device__ __forceinline__ uint32_t chunk_at(int r, int j) {
+  if constexpr (D >= 64)
+    return (j >> 3) * TcCfg<D>::kSub + r * 128 + (((j & 7) ^ (r & 7)) << 4);
+  else
+    return r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>)
+    return f2_to_h2(a, b);
+  else
+    return f2_to_bf2(a, b);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same_v<T, __half>)
+    return h2_to_f2(w);
+  else
+    return bf2_to_f2(w);
+}
+// Whether a pair of 16-bit values holds an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool non_finite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+struct Shared {
+  uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], o_full[2], v_seen[2], drain;
+  uint32_t tmem;
+  int gave_up, skip[2];
+  int poison[2][3];  // non-finite values under a mask, by half; three masked tiles in turn
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_attn_tc_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  griddep_wait();
+  griddep_release();
+  using Cfg = TcCfg<D>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ unsigned char tc_smem[];
+  __shared__ Shared sh;
+  const uint32_t base = (smem_u32(tc_smem) + 1023u) & ~1023u;
+  unsigned char *base_p = tc_smem + (base - smem_u32(tc_smem));
+  const uint32_t kv_base = base + 2 * Cfg::kTile;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int *gave_up = &sh.gave_up;
+
+  const uint32_t kv_full = smem_u32(sh.kv_full), kv_empty = smem_u32(sh.kv_empty), q_full = smem_u32(sh.q_full);
+  const uint32_t s_full = smem_u32(sh.s_full), p_full = smem_u32(sh.p_full), o_full = smem_u32(sh.o_full);
+  const uint32_t v_seen = smem_u32(sh.v_seen);
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(kv_full + 8 * i, 1);
+      mbar_init(kv_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + 8 * i, 128);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 128);
+      mbar_init(o_full + 8 * i, 1);
+      mbar_init(v_seen + 8 * i, 128);
+      sh.skip[i] = sh.poison[i][0] = sh.poison[i][1] = sh.poison[i][2] = 0;
+    }
+    mbar_init(smem_u32(&sh.drain), 1);
+    sh.gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    proxy_fence();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  // Tensor memory: S of the halves at columns 0 and 128 (P over them), O behind.
+  const uint32_t o_col = 256;
+
+  // 384 x 168 registers at launch, split as 2 x 128 x 208 + 128 x 88.
+  Tile t;
+  if (warp >= kLoadWarp) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+   Walk w(a, blockIdx.x);
+   if (warp == kLoadWarp) {
+    const int box_rows = a.page_shift < 7 ? 1 << a.page_shift : 128;
+    const int boxes = 128 / box_rows * Cfg::kHalves;
+    const int box = lane / Cfg::kHalves, half = lane % Cfg::kHalves;  // lanes < boxes issue one load each
+    uint32_t n = 0;  // tiles loaded
+    bool ok = true;
+    for (; ok && w.get(a, t); w.next(a)) {
+      const int64_t hi = t.pos0 + t.ntok, lo = a.window > 0 && t.pos0 - a.window + 1 > 0 ? t.pos0 - a.window + 1 : 0;
+      const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
+      for (int64_t u = u0; ok && u < u0 + w.take; ++u) {
+        const int64_t key = u * kBN + box * box_rows, blk = key >> a.page_shift;
+        int page = static_cast<int>(a.n_pages);  // outside the pool: reads as zeros
+        if (lane < boxes && key < hi && key + box_rows > lo) {
+          const int32_t id = a.table[t.req * a.max_blocks + blk];
+          if (id >= 0 && id < a.n_pages)
+            page = id;
+          else if (a.err_flag != nullptr)
+            atomicOr(a.err_flag, XN_DEVERR_RANGE);
+        }
+        const int row = static_cast<int>(key & ((int64_t{1} << a.page_shift) - 1));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const uint32_t st = n % S, round = n / S;
+          ok = __all_sync(0xffffffffu, round == 0 || wait(kv_empty + 8 * st, (round - 1) & 1, gave_up));
+          if (!ok) break;
+          if (lane == 0) mbar_expect(kv_full + 8 * st, Cfg::kTile);
+          __syncwarp();
+          if (lane < boxes)
+            tma_load(kv_base + st * Cfg::kTile + half * Cfg::kSub + box * box_rows * Cfg::kRowBytes, kv ? &vmap : &kmap,
+                     kv_full + 8 * st, half * 64, row, w.head, page);
+        }
+      }
+    }
+    if (!ok)  // copies in flight end before the block does
+      for (uint32_t i = n > S ? n - S : 0; i < n; ++i) wait(kv_full + 8 * (i % S), (i / S) & 1, gave_up);
+   } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t fmt = std::is_same_v<T, __half> ? 0u : 1u;
+      constexpr uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (128u >> 4) << 24;
+      constexpr uint32_t idesc_s = idesc | (kBN >> 3) << 17;
+      constexpr uint32_t idesc_o = idesc | 1u << 16 | (D >> 3) << 17;  // V: keys are the slow dimension
+      constexpr uint32_t group8 = 8 * Cfg::kRowBytes, hi = desc_hi(group8, D >= 64 ? 2 : 4);
+      uint32_t n = 0, np[2] = {0, 0}, nq[2] = {0, 0};
+      bool ok = true;
+      auto full = [&](uint32_t i) { return wait(kv_full + 8 * (i % S), (i / S) & 1, gave_up); };
+      auto scores = [&](int half, uint32_t i) {  // S[half] = Q[half] K^T, K the i-th tile loaded
+        const uint32_t q = desc_lo(base + half * Cfg::kTile, 16), k = desc_lo(kv_base + (i % S) * Cfg::kTile, 16);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk / 4 * Cfg::kSub + kk % 4 * 32) >> 4;
+          mma_ss(tmem + half * 128, q + off, k + off, hi, idesc_s, kk > 0);
+        }
+        tc_commit(s_full + 8 * half);
+      };
+      auto output = [&](int half, uint32_t i, bool add) {  // O[half] (+)= P[half] V, V the i-th tile loaded
+        const uint32_t v = desc_lo(kv_base + (i % S) * Cfg::kTile, Cfg::kSub);
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          mma_ts(tmem + o_col + half * D, tmem + half * 128 + kk * 8, v + (kk * 2 * group8 >> 4), hi, idesc_o, add || kk > 0);
+      };
+      for (; ok && w.get(a, t); w.next(a)) {
+        const int halves = t.ntok * a.group > 128 ? 2 : 1;
+        ok = full(n);
+        for (int h = 0; ok && h < halves; ++h) {
+          ok = wait(q_full + 8 * h, nq[h]++ & 1, gave_up);
+          if (!ok) break;
+          tc_fence_after();
+          scores(h, n);
+        }
+        if (!ok) break;
+        tc_commit(kv_empty + 8 * (n % S));
+        for (int j = 0; ok && j < w.take; ++j) {
+          const bool more = j + 1 < w.take;
+          for (int h = 0; h < halves; ++h) {
+            ok = wait(p_full + 8 * h, np[h]++ & 1, gave_up) && (h > 0 || (full(n + 1) && (!more || full(n + 2))));
+            if (!ok) break;
+            tc_fence_after();
+            if (!*static_cast<volatile int *>(&sh.skip[h])) output(h, n + 1, j > 0);
+            if (h == halves - 1) tc_commit(kv_empty + 8 * ((n + 1) % S));
+            if (more)
+              scores(h, n + 2);
+            else
+              tc_commit(o_full + 8 * h);
+          }
+          if (ok && more) tc_commit(kv_empty + 8 * ((n + 2) % S));
+          n += 2;
+        }
+      }
+      if (!ok) {  // products in flight end before tensor memory is freed
+        tc_commit(smem_u32(&sh.drain));
+        for (int i = 0; i < 1 << 20 && !mbar_try(smem_u32(&sh.drain), 0); ++i) {
+        }
+      }
+    }
+    __syncwarp();
+   }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    Walk w(a, blockIdx.x);
+    const int h = warp >> 2, wt = tid & 127;  // half, thread of the warpgroup = row of the half
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + h * 128, o_addr = tmem + lanes + o_col + h * D;
+    const float c = a.scale_log2;
+    uint32_t ns = 0, no = 0, nm = 0, units = 0;  // S tiles, items, masked tiles of this half; units of the CTA
+    auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity, gave_up)); };
+    bool ok = true;
+    for (; w.get(a, t); w.next(a)) {
+      const int rows = t.ntok * a.group;
+      const int row = h * 128 + wt;
+      const bool whole = w.whole(t);
+      if (h == 1 && rows <= 128) {
+        units += w.take;
+        continue;
+      }
+      const int64_t pos = t.pos0 + row / a.group;
+      float m = -INFINITY, l = 0.f;
+      if (ok) {
+        // Q: the last item's score products are done (its last s_full was waited for).
+        unsigned char *qs = base_p + h * Cfg::kTile;
+        for (int i = wt; i < 128 * (D / 8); i += 128) {
+          const int r = i / (D / 8), j = i % (D / 8), qr = h * 128 + r;
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (qr < rows) {
+            const int tk = qr / a.group;
+            x = ld_cached(static_cast<const T *>(a.q) + (t.tok0 + tk) * a.q_stride + (w.head * a.group + qr - tk * a.group) * D + j * 8);
+          }
+          *reinterpret_cast<uint4 *>(qs + chunk_at<D>(r, j)) = x;
+        }
+        proxy_fence();
+        mbar_arrive(q_full + 8 * h);
+      }
+      const int64_t hi = t.pos0 + t.ntok, lo = a.window > 0 && t.pos0 - a.window + 1 > 0 ? t.pos0 - a.window + 1 : 0;
+      const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
+      for (int j = 0; ok && j < w.take; ++j, ++units) {
+        const int64_t key0 = (u0 + j) * kBN;
+        const bool masked = key0 + kBN - 1 > t.pos0 || (a.window > 0 && key0 <= hi - 1 - a.window);
+        int seen_lo = 0, seen_hi = kBN;  // keys of the tile that this row sees
+        if (masked) {
+          const int64_t e = pos + 1 - key0, b = a.window > 0 ? e - a.window : 0;
+          seen_hi = static_cast<int>(e < 0 ? 0 : e > kBN ? kBN : e);
+          seen_lo = static_cast<int>(b < 0 ? 0 : b > kBN ? kBN : b);
+        }
+        ok = all_wait(s_full + 8 * h, ns++ & 1);
+        if (!ok) break;
+        tc_fence_after();
+        float s[kBN];
+#pragma unroll
+        for (int i = 0; i < kBN; i += 32) tc_ld32(s_addr + i, s + i);
+        tc_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < kBN; ++i) s[i] = i >= seen_lo && i < seen_hi ? s[i] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < kBN; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // A larger maximum by more than 2^8: this warp's rows move to it.
+        if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
+          const float to = fmaxf(m, top), f = m == to ? 1.f : ex2_approx_ftz((m - to) * c);
+          m = to;
+          l *= f;
+          if (j > 0) {
+#pragma unroll
+            for (int i = 0; i < D; i += 32) {
+              float o[32];
+              tc_ld32(o_addr + i, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] *= f;
+              tc_st32(o_addr + i, reinterpret_cast<uint32_t *>(o));
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.f : -m * c;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t p[kBN / 2];
+#pragma unroll
+        for (int i = 0; i < kBN; i += 2) {
+          const float x = ex2_approx_ftz(__fmaf_rn(s[i], c, mc)), y = ex2_approx_ftz(__fmaf_rn(s[i + 1], c, mc));
+          sum[i & 3] += x;
+          sum[(i + 1) & 3] += y;
+          p[i / 2] = pack2<T>(x, y);
+        }
+        tc_st32(s_addr, p);
+        tc_st32(s_addr + 32, p + 32);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        int poisoned = 0;
+        if (masked) {
+          const uint32_t nv = 2 * units + 1;
+          ok = all_wait(kv_full + 8 * (nv % S), (nv / S) & 1);
+          if (!ok) break;
+          unsigned char *vs = base_p + 2 * Cfg::kTile + (nv % S) * Cfg::kTile;
+          const int64_t key = key0 + wt;  // this thread's V row
+          bool bad = false;
+          if (key >= hi || key < lo) {
+            for (int q = 0; q < D / 8; ++q) *reinterpret_cast<uint4 *>(vs + chunk_at<D>(wt, q)) = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            for (int q = 0; q < D / 8; ++q) {
+              const uint4 x = *reinterpret_cast<const uint4 *>(vs + chunk_at<D>(wt, q));
+              bad |= non_finite2<T>(x.x) | non_finite2<T>(x.y) | non_finite2<T>(x.z) | non_finite2<T>(x.w);
+            }
+          }
+          proxy_fence();
+          // The half's 128 threads agree. Slots are used in turn: the next one is
+          // cleared when everyone has read its last use (before the wait just passed).
+          volatile int *poison = sh.poison[h];
+          if (bad) poison[nm % 3] = 1;
+          if (wt == 0) poison[(nm + 1) % 3] = 0;
+          mbar_arrive(v_seen + 8 * h);
+          ok = all_wait(v_seen + 8 * h, nm & 1);
+          if (!ok) break;
+          poisoned = poison[nm++ % 3];
+          if (poisoned) {
+            tc_wait_st();
+#pragma unroll 1
+            for (int i = 0; i < D; i += 32) {
+              float o[32];
+              if (j > 0) {
+                tc_ld32(o_addr + i, o);
+                tc_wait_ld();
+              } else {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = 0.f;
+              }
+#pragma unroll 1
+              for (int kb = 0; kb < kBN; kb += 8) {
+                uint32_t pw[4];
+                __syncwarp();
+                tc_ld4(s_addr + kb / 2, pw);
+                tc_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  if (kb + k < seen_lo || kb + k >= seen_hi) continue;
+                  const float2 p2 = unpack2<T>(pw[k / 2]);
+                  const float pk = k & 1 ? p2.y : p2.x;
+#pragma unroll
+                  for (int q = 0; q < 4; ++q) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(vs + chunk_at<D>(kb + k, i / 8 + q));
+                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                      const float2 v2 = unpack2<T>(xw[e]);
+                      o[q * 8 + e * 2] = __fmaf_rn(pk, v2.x, o[q * 8 + e * 2]);
+                      o[q * 8 + e * 2 + 1] = __fmaf_rn(pk, v2.y, o[q * 8 + e * 2 + 1]);
+                    }
+                  }
+                }
+              }
+              __syncwarp();
+              tc_st32(o_addr + i, reinterpret_cast<uint32_t *>(o));
+            }
+          }
+        }
+        if (wt == 0) *static_cast<volatile int *>(&sh.skip[h]) = poisoned;
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full + 8 * h);
+      }
+      if (ok) ok = all_wait(o_full + 8 * h, no++ & 1);
+      if (!ok && wt == 0 && a.err_flag != nullptr) atomicOr(a.err_flag, XN_DEVERR_WAIT);
+      tc_fence_after();
+      // Rows out: a thread writes its row. After a wait that gave up: NaN.
+      const float nan = __int_as_float(0x7fc00000);
+      float *part_o = partial_of(a, blockIdx.x, w.first ? 0 : 1, kBM, D);
+      const int tk = row / a.group;
+      T *dst = static_cast<T *>(a.out) + (static_cast<int64_t>(t.tok0 + tk) * a.h + w.head * a.group + row - tk * a.group) * D;
+      const float inv = __fdiv_rn(1.f, l);
+#pragma unroll
+      for (int i = 0; i < D; i += 32) {
+        float o[32];
+        __syncwarp();
+        if (ok) {
+          tc_ld32(o_addr + i, o);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = nan;
+        }
+        if (row >= rows) continue;
+        if (whole) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = pos < 0 ? 0.f : o[k] * inv;
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            st_vec(dst + i + k, make_uint4(pack2<T>(o[k], o[k + 1]), pack2<T>(o[k + 2], o[k + 3]), pack2<T>(o[k + 4], o[k + 5]),
+                                           pack2<T>(o[k + 6], o[k + 7])));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *reinterpret_cast<float4 *>(part_o + row * D + i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        }
+      }
+      if (!whole && row < rows) {
+        part_o[kBM * D + row] = ok ? m : nan;
+        part_o[kBM * D + kBM + row] = ok ? l : nan;
+      }
+      tc_fence_before();  // O is read before the next item's products write it
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &res) != cudaSuccess ||
+        res != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// A pool as a 4-D tensor (d, slot, head, page); a box is `rows` slots of one page and head.
+bool make_map(CUtensorMap *map, const void *pool, const Args &a, int d, int page_size, bool bf16) {
+  EncodeFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(page_size), static_cast<cuuint64_t>(a.h_kv),
+                              static_cast<cuuint64_t>(a.n_pages)};
+  // A dimension of one element may come with any stride: give it a valid one.
+  const int64_t ss = page_size > 1 ? a.slot_stride : d, hs = a.h_kv > 1 ? a.head_stride : ss * page_size;
+  const int64_t ps = a.n_pages > 1 ? a.page_stride : ss * page_size;
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(ss) * 2, static_cast<cuuint64_t>(hs) * 2, static_cast<cuuint64_t>(ps) * 2};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(d < 64 ? d : 64), static_cast<cuuint32_t>(page_size < 128 ? page_size : 128), 1, 1};
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(pool), dims,
+            strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, d < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+int launch(const Args &a, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t st, const char *op) {
+  constexpr int smem = static_cast<int>(TcCfg<D>::kSmem);
+  if (cudaFuncSetAttribute(paged_attn_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return check_launch(op);
+  launch_k(paged_attn_tc_kernel<T, D>, dim3(a.parts), dim3(kThreads), smem, st, a, kmap, vmap);
+  return XN_OK;
+}
+
+}  // namespace
+
+int launch_tc(const Args &a, int d, int dtype, cudaStream_t st, const char *op) {
+  CUtensorMap kmap, vmap;
+  const bool bf16 = dtype == XN_BF16;
+  if (!make_map(&kmap, a.k, a, d, 1 << a.page_shift, bf16) || !make_map(&vmap, a.v, a, d, 1 << a.page_shift, bf16))
+    return fail(XN_E_CUDA, "%s: the driver refused a tensor map of the pools", op);
+  if (bf16) {
+    if (d == 32) return launch<__nv_bfloat16, 32>(a, kmap, vmap, st, op);
+    if (d == 64) return launch<__nv_bfloat16, 64>(a, kmap, vmap, st, op);
+    return launch<__nv_bfloat16, 128>(a, kmap, vmap, st, op);
+  }
+  if (d == 32) return launch<__half, 32>(a, kmap, vmap, st, op);
+  if (d == 64) return launch<__half, 64>(a, kmap, vmap, st, op);
+  return launch<__half, 128>(a, kmap, vmap, st, op);
+}
+
+}  // namespace paged
+}  // namespace xn
