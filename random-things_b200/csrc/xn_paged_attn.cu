@@ -127,10 +127,11 @@ struct SimtCfg {
   static constexpr size_t kSmem = sizeof(float) * (kQ + kK + kV + kP);
 };
 
-template <typename T, int D, int BM>
+template <int D, int BM>
 __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
   griddep_wait();
   griddep_release();
+  using T = float;
   using Cfg = SimtCfg<D, BM>;
   constexpr int BN = Cfg::kBN, R = Cfg::kRows, V = Elem<T>::kVec, CP = D / 16;
   extern __shared__ __align__(16) float simt_smem[];
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
       for (int c = 0; c < CP; ++c) o[r][c] = 0.f;
     }
     const int64_t key_hi = t.pos0 + t.ntok;  // keys from here on are seen by no row
-    const int64_t key_lo = a.window > 0 ? t.pos0 - a.window + 1 : 0;
+    const int64_t lo = key_lo(t, a.window);
     const int64_t u0 = first_unit(t, a.window, BN) + w.k;
     for (int64_t u = u0; u < u0 + w.take; ++u) {
       const int64_t key0 = u * BN;
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
         const int row = i / (D / V), c = i % (D / V) * V;
         const int64_t key = key0 + row;
         float kx[V] = {}, vx[V] = {};
-        if (key < key_hi && key >= key_lo) {
+        if (key < key_hi && key >= lo) {
           const int32_t page = a.table[t.req * a.max_blocks + (key >> a.page_shift)];
           if (page >= 0 && page < a.n_pages) {
             const int64_t at = page * a.page_stride + w.head * a.head_stride + (key & page_mask) * a.slot_stride + c;
@@ -342,8 +343,8 @@ struct Shape {
 
 Shape shape_of(int64_t group, int64_t max_new, int dtype) {
   const bool few = max_new * group <= 16 && group <= 16;
-  if (!few && dtype != XN_F32) return Shape{kTcRows, kTcKeys, sm_count(), 2};
-  return Shape{few ? 16 : 64, 64, 2 * sm_count(), 4};
+  if (dtype == XN_F32) return Shape{few ? 16 : 64, 64, 2 * sm_count(), 4};
+  return few ? Shape{kDecRows, kDecKeys, 2 * sm_count(), 4} : Shape{kTcRows, kTcKeys, sm_count(), 2};
 }
 
 struct Layout {
@@ -361,23 +362,25 @@ Layout layout_of(const Shape &s, int64_t n_tokens, int64_t requests, int64_t gro
   return l;
 }
 
-template <typename T, int D, int BM>
+template <int D, int BM>
 void launch_simt(const Args &a, cudaStream_t st) {
   constexpr size_t smem = SimtCfg<D, BM>::kSmem;
-  cudaFuncSetAttribute(paged_attn_simt_kernel<T, D, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  launch_k(paged_attn_simt_kernel<T, D, BM>, dim3(a.parts), dim3(256), smem, st, a);
+  cudaFuncSetAttribute(paged_attn_simt_kernel<D, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  launch_k(paged_attn_simt_kernel<D, BM>, dim3(a.parts), dim3(256), smem, st, a);
 }
 
 template <typename T, int D>
 int launch_attn(const Args &a, const Shape &s, cudaStream_t st, const char *op) {
   const size_t smem = sizeof(int32_t) * (static_cast<size_t>(a.requests) + 1);
   launch_k(paged_schedule_kernel, dim3(1), dim3(kSchedThreads), smem, st, a);
-  if (s.bm == kTcRows) {
-    if (const int rc = launch_tc(a, D, std::is_same_v<T, float> ? XN_F32 : std::is_same_v<T, __half> ? XN_F16 : XN_BF16, st, op)) return rc;
-  } else if (s.bm == 16) {
-    launch_simt<T, D, 16>(a, st);
-  } else if constexpr (std::is_same_v<T, float>) {
-    launch_simt<T, D, 64>(a, st);
+  if constexpr (std::is_same_v<T, float>) {
+    if (s.bm == 16)
+      launch_simt<D, 16>(a, st);
+    else
+      launch_simt<D, 64>(a, st);
+  } else {
+    constexpr int dtype = std::is_same_v<T, __half> ? XN_F16 : XN_BF16;
+    if (const int rc = s.bm == kTcRows ? launch_tc(a, D, dtype, st, op) : launch_dec(a, D, dtype, st, op)) return rc;
   }
   if (a.parts > 1) launch_k(paged_combine_kernel<T, D>, dim3(a.parts - 1, ceil_div(s.bm, 16)), dim3(128), 0, st, a, s.bm);
   return check_launch(op);

@@ -53,11 +53,12 @@ struct Args {
   float *partial;  // 2 * parts records
 };
 
-// First key tile that a query tile's rows see.
-__device__ __forceinline__ int64_t first_unit(const Tile &t, int64_t window, int bn) {
+// First key that a query tile's rows see, and its key tile.
+__device__ __forceinline__ int64_t key_lo(const Tile &t, int64_t window) {
   const int64_t lo = t.pos0 - window + 1;
-  return window > 0 && lo > 0 ? lo / bn : 0;
+  return window > 0 && lo > 0 ? lo : 0;
 }
+__device__ __forceinline__ int64_t first_unit(const Tile &t, int64_t window, int bn) { return key_lo(t, window) / bn; }
 
 // Record of part c's partial sums: [rows][D] of O, then rows maxima, rows sums.
 // Part c has two: 0 for the segment it begins with, 1 for its last one.

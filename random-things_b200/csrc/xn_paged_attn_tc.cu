@@ -24,12 +24,7 @@
 // on the CUDA cores, each token over its own keys (poisoned tile).
 //
 // Every wait has a time limit; see wait().
-#include <cuda.h>
-
-#include <type_traits>
-
-#include "xn_paged_attn.cuh"
-#include "xn_paged_attn_tc.h"
+#include "xn_paged_tma.cuh"
 
 namespace xn {
 namespace paged {
@@ -37,57 +32,13 @@ namespace {
 
 constexpr int kBM = kTcRows, kBN = kTcKeys, kThreads = 384;
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
-constexpr uint64_t kWaitNs = 2000000000ull;  // a wait gives up after 2 s
 
 template <int D>
-struct TcCfg {
-  static constexpr int kRowBytes = D >= 64 ? 128 : 64;    // bytes of a swizzled row
-  static constexpr int kHalves = D >= 64 ? D / 64 : 1;    // sub-tiles of kRowBytes a row
-  static constexpr int kSub = 128 * kRowBytes;            // bytes of one sub-tile of 128 rows
-  static constexpr int kTile = kHalves * kSub;            // a Q half, a K tile or a V tile
+struct TcCfg : Swizzled<D, 128> {  // a Q half, a K tile and a V tile have 128 rows
+  using Swizzled<D, 128>::kTile;
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr size_t kSmem = 1024 + 2 * kTile + kStages * kTile;
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Waits for the phase of `parity`; false when it did not come within kWaitNs or
-// another role gave up (then nothing that the phase stands for may be used).
-// Inlined: with a call in the kernel its register split would not take effect.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
-  uint64_t t0 = 0, t;
-  while (true) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try(bar, parity)) return true;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t0 == 0) t0 = t;
-    if (*gave_up || t - t0 > kWaitNs) break;
-  }
-  *gave_up = 1;
-  return false;
-}
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -96,7 +47,6 @@ __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // 32 columns of this warp's 32 lanes (one lane a row) from / to tensor memory.
 __device__ __forceinline__ void tc_ld32(uint32_t addr, float *r) {
@@ -144,51 +94,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int row, int head,
-                                         int page) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
-          dst),
-      "l"(map), "r"(bar), "r"(x), "r"(row), "r"(head), "r"(page)
-      : "memory");
-}
-
 // Shared-memory operand descriptor. Low word: address and leading byte offset
 // in 16-byte units (so a step of n bytes adds n / 16; addresses stay below
 // 2^18); high word: stride byte offset, version 1, swizzle of 128 (code 2) or
 // 64 bytes (code 4).
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return addr >> 4 | (lbo >> 4) << 16; }
 constexpr uint32_t desc_hi(uint32_t sbo, uint32_t swizzle) { return sbo >> 4 | 1u << 14 | swizzle << 29; }
-
-// Byte offset of 16-byte chunk j of row r in a swizzled tile.
-template <int D>
-__device__ __forceinline__ uint32_t chunk_at(int r, int j) {
-  if constexpr (D >= 64)
-    return (j >> 3) * TcCfg<D>::kSub + r * 128 + (((j & 7) ^ (r & 7)) << 4);
-  else
-    return r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __half>)
-    return f2_to_h2(a, b);
-  else
-    return f2_to_bf2(a, b);
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (std::is_same_v<T, __half>)
-    return h2_to_f2(w);
-  else
-    return bf2_to_f2(w);
-}
-// Whether a pair of 16-bit values holds an infinity or NaN.
-template <typename T>
-__device__ __forceinline__ bool non_finite2(uint32_t w) {
-  constexpr uint32_t e = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || ((w >> 16) & e) == e;
-}
 
 struct Shared {
   uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], o_full[2], v_seen[2], drain;
@@ -250,25 +161,14 @@ __global__ void __launch_bounds__(kThreads, 1)
    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
    Walk w(a, blockIdx.x);
    if (warp == kLoadWarp) {
-    const int box_rows = a.page_shift < 7 ? 1 << a.page_shift : 128;
-    const int boxes = 128 / box_rows * Cfg::kHalves;
-    const int box = lane / Cfg::kHalves, half = lane % Cfg::kHalves;  // lanes < boxes issue one load each
+    const TileLoad<D, kBN> ld(a);
     uint32_t n = 0;  // tiles loaded
     bool ok = true;
     for (; ok && w.get(a, t); w.next(a)) {
-      const int64_t hi = t.pos0 + t.ntok, lo = a.window > 0 && t.pos0 - a.window + 1 > 0 ? t.pos0 - a.window + 1 : 0;
+      const int64_t hi = t.pos0 + t.ntok, lo = key_lo(t, a.window);
       const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
       for (int64_t u = u0; ok && u < u0 + w.take; ++u) {
-        const int64_t key = u * kBN + box * box_rows, blk = key >> a.page_shift;
-        int page = static_cast<int>(a.n_pages);  // outside the pool: reads as zeros
-        if (lane < boxes && key < hi && key + box_rows > lo) {
-          const int32_t id = a.table[t.req * a.max_blocks + blk];
-          if (id >= 0 && id < a.n_pages)
-            page = id;
-          else if (a.err_flag != nullptr)
-            atomicOr(a.err_flag, XN_DEVERR_RANGE);
-        }
-        const int row = static_cast<int>(key & ((int64_t{1} << a.page_shift) - 1));
+        const int page = ld.page(a, t, u * kBN, lo, hi);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++n) {
           const uint32_t st = n % S, round = n / S;
@@ -276,9 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           if (lane == 0) mbar_expect(kv_full + 8 * st, Cfg::kTile);
           __syncwarp();
-          if (lane < boxes)
-            tma_load(kv_base + st * Cfg::kTile + half * Cfg::kSub + box * box_rows * Cfg::kRowBytes, kv ? &vmap : &kmap,
-                     kv_full + 8 * st, half * 64, row, w.head, page);
+          ld.load(a, kv ? &vmap : &kmap, kv_base + st * Cfg::kTile, kv_full + 8 * st, u * kBN, w.head, page);
         }
       }
     }
@@ -375,12 +273,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int tk = qr / a.group;
             x = ld_cached(static_cast<const T *>(a.q) + (t.tok0 + tk) * a.q_stride + (w.head * a.group + qr - tk * a.group) * D + j * 8);
           }
-          *reinterpret_cast<uint4 *>(qs + chunk_at<D>(r, j)) = x;
+          *reinterpret_cast<uint4 *>(qs + Cfg::chunk_at(r, j)) = x;
         }
         proxy_fence();
         mbar_arrive(q_full + 8 * h);
       }
-      const int64_t hi = t.pos0 + t.ntok, lo = a.window > 0 && t.pos0 - a.window + 1 > 0 ? t.pos0 - a.window + 1 : 0;
+      const int64_t hi = t.pos0 + t.ntok, lo = key_lo(t, a.window);
       const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
       for (int j = 0; ok && j < w.take; ++j, ++units) {
         const int64_t key0 = (u0 + j) * kBN;
@@ -445,10 +343,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t key = key0 + wt;  // this thread's V row
           bool bad = false;
           if (key >= hi || key < lo) {
-            for (int q = 0; q < D / 8; ++q) *reinterpret_cast<uint4 *>(vs + chunk_at<D>(wt, q)) = make_uint4(0u, 0u, 0u, 0u);
+            for (int q = 0; q < D / 8; ++q) *reinterpret_cast<uint4 *>(vs + Cfg::chunk_at(wt, q)) = make_uint4(0u, 0u, 0u, 0u);
           } else {
             for (int q = 0; q < D / 8; ++q) {
-              const uint4 x = *reinterpret_cast<const uint4 *>(vs + chunk_at<D>(wt, q));
+              const uint4 x = *reinterpret_cast<const uint4 *>(vs + Cfg::chunk_at(wt, q));
               bad |= non_finite2<T>(x.x) | non_finite2<T>(x.y) | non_finite2<T>(x.z) | non_finite2<T>(x.w);
             }
           }
@@ -487,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const float pk = k & 1 ? p2.y : p2.x;
 #pragma unroll
                   for (int q = 0; q < 4; ++q) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(vs + chunk_at<D>(kb + k, i / 8 + q));
+                    const uint4 x = *reinterpret_cast<const uint4 *>(vs + Cfg::chunk_at(kb + k, i / 8 + q));
                     const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -555,39 +453,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult res;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &res) != cudaSuccess ||
-        res != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeFn>(p);
-  }();
-  return fn;
-}
-
-// A pool as a 4-D tensor (d, slot, head, page); a box is `rows` slots of one page and head.
-bool make_map(CUtensorMap *map, const void *pool, const Args &a, int d, int page_size, bool bf16) {
-  EncodeFn fn = encode_fn();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(page_size), static_cast<cuuint64_t>(a.h_kv),
-                              static_cast<cuuint64_t>(a.n_pages)};
-  // A dimension of one element may come with any stride: give it a valid one.
-  const int64_t ss = page_size > 1 ? a.slot_stride : d, hs = a.h_kv > 1 ? a.head_stride : ss * page_size;
-  const int64_t ps = a.n_pages > 1 ? a.page_stride : ss * page_size;
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(ss) * 2, static_cast<cuuint64_t>(hs) * 2, static_cast<cuuint64_t>(ps) * 2};
-  const cuuint32_t box[4] = {static_cast<cuuint32_t>(d < 64 ? d : 64), static_cast<cuuint32_t>(page_size < 128 ? page_size : 128), 1, 1};
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(pool), dims,
-            strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, d < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int D>
 int launch(const Args &a, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t st, const char *op) {
   constexpr int smem = static_cast<int>(TcCfg<D>::kSmem);
@@ -602,7 +467,7 @@ int launch(const Args &a, const CUtensorMap &kmap, const CUtensorMap &vmap, cuda
 int launch_tc(const Args &a, int d, int dtype, cudaStream_t st, const char *op) {
   CUtensorMap kmap, vmap;
   const bool bf16 = dtype == XN_BF16;
-  if (!make_map(&kmap, a.k, a, d, 1 << a.page_shift, bf16) || !make_map(&vmap, a.v, a, d, 1 << a.page_shift, bf16))
+  if (!make_map(&kmap, a.k, a, d, kBN, bf16) || !make_map(&vmap, a.v, a, d, kBN, bf16))
     return fail(XN_E_CUDA, "%s: the driver refused a tensor map of the pools", op);
   if (bf16) {
     if (d == 32) return launch<__nv_bfloat16, 32>(a, kmap, vmap, st, op);

@@ -1,4 +1,4 @@
-// xn_paged_attn_tc.h - host entry of the tensor-core kernel of the paged attention.
+// xn_paged_attn_tc.h - host entries of the paged attention's tensor-core kernels.
 #pragma once
 
 #include "xn_paged_attn.cuh"
@@ -6,10 +6,13 @@
 namespace xn {
 namespace paged {
 
-constexpr int kTcRows = 256, kTcKeys = 128;  // rows of a query tile, keys of a key tile
+// Rows of a query tile and keys of a key tile: chunks, and single tokens.
+constexpr int kTcRows = 256, kTcKeys = 128;
+constexpr int kDecRows = 16, kDecKeys = 64;
 
-// Enqueues the kernel (bf16 / f16); XN_OK, or the error recorded.
+// Enqueue the kernel for chunks / for single tokens (bf16 / f16); XN_OK, or the error recorded.
 int launch_tc(const Args &a, int d, int dtype, cudaStream_t st, const char *op);
+int launch_dec(const Args &a, int d, int dtype, cudaStream_t st, const char *op);
 
 }  // namespace paged
 }  // namespace xn
