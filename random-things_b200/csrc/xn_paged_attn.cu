@@ -91,27 +91,27 @@ __global__ void __launch_bounds__(kSchedThreads) paged_schedule_kernel(const Arg
       const int64_t u = end <= 0 ? 1 : (end + a.bn - 1) / a.bn - first_unit(t, a.window, a.bn);
       t.units = static_cast<int32_t>(u);
     }
-    t.ustart = carry + block_scan_excl(t.units, tot, all);
+    t.cstart = carry + block_scan_excl(e < n_tiles ? t.units + a.pair_cost : 0, tot, all);
     carry += all;
     if (e < n_tiles) a.tiles[e] = t;
   }
   const int64_t w = carry * a.h_kv;
-  int64_t ctas = (w + a.min_units - 1) / a.min_units;
+  int64_t ctas = (w + a.min_cost - 1) / a.min_cost;
   if (ctas > a.parts) ctas = a.parts;
   if (tid == 0) {
-    a.header->n_tiles = n_tiles;
-    a.header->units = w;
     a.header->ctas = static_cast<int32_t>(ctas);
+    a.starts[ctas] = Start{static_cast<int32_t>(n_tiles), 0, 0, 0};
   }
-  // The thread that holds a tile marks the parts that begin in it.
+  // The thread that holds a tile marks the parts that begin in it. A cut in
+  // what a pair costs beyond its units moves to the pair's begin.
   for (int64_t e = tid; e < n_tiles; e += kSchedThreads) {
     const Tile t = a.tiles[e];
-    const int64_t lo = t.ustart * a.h_kv, hi = lo + static_cast<int64_t>(t.units) * a.h_kv;
+    const int64_t pair = t.units + a.pair_cost, lo = t.cstart * a.h_kv, hi = lo + pair * a.h_kv;
     for (int64_t c = (lo * ctas + w - 1) / w; c < ctas; ++c) {
-      const int64_t at = c * w / ctas;
-      if (at >= hi) break;
-      const int64_t r = at - lo;
-      a.starts[c] = Start{static_cast<int32_t>(e), static_cast<int32_t>(r / t.units), static_cast<int32_t>(r % t.units), 0};
+      const int64_t r = c * w / ctas - lo;
+      if (r >= hi - lo) break;
+      const int64_t k = r % pair - a.pair_cost;
+      a.starts[c] = Start{static_cast<int32_t>(e), static_cast<int32_t>(r / pair), static_cast<int32_t>(k > 0 ? k : 0), 0};
     }
   }
 }
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kSchedThreads) paged_schedule_kernel(const Arg
 // ---------------------------------------------------------------------------
 template <int D, int BM>
 struct SimtCfg {
-  static constexpr int kBN = 64, kThreads = 256, kRows = BM / 16;
+  static constexpr int kBN = 64, kRows = BM / 16;
   static constexpr int kQ = BM * D, kK = kBN * (D + 4), kV = kBN * D, kP = BM * (kBN + 4);
   static constexpr size_t kSmem = sizeof(float) * (kQ + kK + kV + kP);
 };
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
       const int row = i / (D / V), c = i % (D / V) * V;
       float x[V] = {};
       if (row < rows) {
-        const int64_t tok = t.tok0 + row / a.group, head = w.head * a.group + row % a.group;
+        const int64_t tok = t.tok0 + token_of(a, row), head = w.head * a.group + row - token_of(a, row) * a.group;
         unpack<T>(ld_cached(static_cast<const T *>(a.q) + tok * a.q_stride + head * D + c), x);
       }
 #pragma unroll
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
     for (int r = 0; r < R; ++r) {
       m[r] = -INFINITY;
       l[r] = 0.f;
-      pos[r] = t.pos0 + (ty * R + r) / a.group;
+      pos[r] = t.pos0 + token_of(a, ty * R + r);
 #pragma unroll
       for (int c = 0; c < CP; ++c) o[r][c] = 0.f;
     }
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
       const int row = ty * R + r;
       if (row >= rows) continue;
       const float inv = pos[r] < 0 ? 0.f : __fdiv_rn(1.f, l[r]);
-      const int64_t tok = t.tok0 + row / a.group, head = w.head * a.group + row % a.group;
+      const int64_t tok = t.tok0 + token_of(a, row), head = w.head * a.group + row - token_of(a, row) * a.group;
       T *dst = static_cast<T *>(a.out) + (tok * a.h + head) * D;
 #pragma unroll
       for (int c = 0; c < CP; ++c) {
@@ -326,10 +326,10 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const Args a, int bm
       o.z = __fmaf_rn(x.z, f, o.z);
       o.w = __fmaf_rn(x.w, f, o.w);
     }
-    const int64_t pos = t.pos0 + row / a.group;
+    const int64_t pos = t.pos0 + token_of(a, row);
     const float inv = __fdiv_rn(1.f, l);
     const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    const int64_t tok = t.tok0 + row / a.group, head = s.head * a.group + row % a.group;
+    const int64_t tok = t.tok0 + token_of(a, row), head = s.head * a.group + row - token_of(a, row) * a.group;
     T *dst = static_cast<T *>(a.out) + (tok * a.h + head) * D + col;
 #pragma unroll
     for (int j = 0; j < 4; ++j) dst[j] = Elem<T>::from_f32(pos < 0 ? 0.f : y[j]);
@@ -338,13 +338,13 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const Args a, int bm
 
 // How a call is cut: rows of a query tile, keys of a key tile, parts.
 struct Shape {
-  int bm, bn, parts, min_units;
+  int bm, bn, parts, pair_cost, min_cost;
 };
 
 Shape shape_of(int64_t group, int64_t max_new, int dtype) {
   const bool few = max_new * group <= 16 && group <= 16;
-  if (dtype == XN_F32) return Shape{few ? 16 : 64, 64, 2 * sm_count(), 4};
-  return few ? Shape{kDecRows, kDecKeys, 2 * sm_count(), 4} : Shape{kTcRows, kTcKeys, sm_count(), 2};
+  if (dtype == XN_F32) return Shape{few ? 16 : 64, 64, 2 * sm_count(), 1, 4};
+  return few ? Shape{kDecRows, kDecKeys, 2 * sm_count(), 2, 6} : Shape{kTcRows, kTcKeys, sm_count(), 3, 5};
 }
 
 struct Layout {
@@ -468,11 +468,13 @@ int xn_paged_attention(void *out, const void *q, const void *k_pages, const void
   a.h = static_cast<int32_t>(h);
   a.h_kv = static_cast<int32_t>(h_kv);
   a.group = static_cast<int32_t>(group);
+  a.group_mul = static_cast<int32_t>((65535 + group) / group);
   a.page_shift = shift;
   a.tile_tokens = static_cast<int32_t>(s.bm / group);
   a.bn = s.bn;
   a.parts = s.parts;
-  a.min_units = s.min_units;
+  a.pair_cost = s.pair_cost;
+  a.min_cost = s.min_cost;
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   a.err_flag = err_flag;
   a.header = reinterpret_cast<paged::Header *>(ws);

@@ -3,15 +3,16 @@
 //
 // Work. A query tile is up to `tile_tokens` consecutive new tokens of one
 // request with the group of query heads that share a kv head: rows (token,
-// head of the group), token-major. A unit is one key tile of kBN keys against
-// one (query tile, kv head). The units of all (tile, head) pairs, in that
-// order, form one line, which is cut into equal parts, one per CTA, wherever
-// the cuts fall: lengths are known on the device only, and equal parts keep
-// every SM busy for ragged batches and for one long request alike. A CTA
-// walks its part as segments, one per (tile, head) it touches. A segment that
-// covers all units of its pair writes the output; the others write partial
-// sums (unnormalised O, row maximum, row sum), which the combine kernel adds
-// in key order: no atomics, and a result that depends on the inputs alone.
+// head of the group), token-major. A unit is one key tile against one (query
+// tile, kv head). The units of all (tile, head) pairs, in that order, form one
+// line, which is cut into parts of equal cost, one per CTA, wherever the cuts
+// fall: lengths are known on the device only, and equal parts keep every SM
+// busy for ragged batches and for one long request alike. A pair costs its
+// units and `pair_cost` more for its query rows and output. A CTA walks its
+// part as segments, one per pair it touches. A segment that covers all units
+// of its pair writes the output; the others write partial sums (unnormalised
+// O, row maximum, row sum), which the combine kernel adds in key order: no
+// atomics, and a result that depends on the inputs alone.
 #pragma once
 
 #include "xn_common.cuh"
@@ -24,7 +25,7 @@ struct Tile {
   int32_t req, tok0, ntok;  // request, its first row of q, tokens in the tile
   int32_t units;            // key tiles that its rows see (at least 1)
   int64_t pos0;             // position of the first token; negative: it sees no key
-  int64_t ustart;           // units of the tiles before it (for one kv head)
+  int64_t cstart;           // cost of the tiles before it (for one kv head)
 };
 
 struct Start {
@@ -33,8 +34,7 @@ struct Start {
 };
 
 struct Header {
-  int64_t n_tiles, units;  // units: of all heads
-  int32_t ctas, pad;       // parts in use
+  int32_t ctas;  // parts in use
 };
 
 struct Args {
@@ -43,13 +43,13 @@ struct Args {
   const int32_t *table;
   const int64_t *q_start, *kv_len;
   int64_t n_tokens, n_pages, max_blocks, q_stride, page_stride, head_stride, slot_stride, window;
-  int32_t requests, h, h_kv, group, page_shift;
-  int32_t tile_tokens, bn, parts, min_units;
+  int32_t requests, h, h_kv, group, group_mul, page_shift;
+  int32_t tile_tokens, bn, parts, pair_cost, min_cost;
   float scale_log2;  // scale * log2(e): scores enter exp2
   int *err_flag;
   Header *header;
   Tile *tiles;
-  Start *starts;  // parts + 1
+  Start *starts;  // of the parts in use, and the end of the last
   float *partial;  // 2 * parts records
 };
 
@@ -66,36 +66,36 @@ __device__ __forceinline__ float *partial_of(const Args &a, int part, int which,
   return a.partial + (static_cast<int64_t>(part) * 2 + which) * (static_cast<int64_t>(rows) * (d + 2));
 }
 
+// Token of a query tile's row: row / group for row < 256, group <= 64.
+__device__ __forceinline__ int token_of(const Args &a, int row) { return row * a.group_mul >> 16; }
+
 // The segments of one CTA's part, in order.
 struct Walk {
-  int64_t left;  // units left in the part
-  int32_t tile, head, k, take;
+  int32_t tile, head, k, take;  // the segment: key tiles k .. k + take - 1 of (tile, head)
+  Start end;
   bool first;
 
   __device__ __forceinline__ Walk(const Args &a, int part) {
-    const int64_t w = a.header->units;
-    const int ctas = a.header->ctas;
-    left = 0;
+    tile = head = k = take = 0;
+    end = Start{0, 0, 0, 0};
     first = true;
-    take = 0;
-    if (part >= ctas) return;
-    left = (part + 1) * w / ctas - part * w / ctas;
+    if (part >= a.header->ctas) return;
     const Start s = a.starts[part];
     tile = s.tile;
     head = s.head;
     k = s.k;
+    end = a.starts[part + 1];
   }
   // Loads the tile of the current segment; false when the part is done.
   __device__ __forceinline__ bool get(const Args &a, Tile &t) {
-    if (left <= 0) return false;
+    const bool same = tile == end.tile && head == end.head;
+    if (tile > end.tile || (tile == end.tile && head > end.head) || (same && k >= end.k)) return false;
     t = a.tiles[tile];
-    const int64_t rest = t.units - k;
-    take = static_cast<int32_t>(rest < left ? rest : left);
+    take = (same ? end.k : t.units) - k;
     return true;
   }
   __device__ __forceinline__ bool whole(const Tile &t) const { return k == 0 && take == t.units; }
   __device__ __forceinline__ void next(const Args &a) {
-    left -= take;
     k = 0;
     first = false;
     if (++head == a.h_kv) {

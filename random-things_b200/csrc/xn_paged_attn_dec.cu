@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     int64_t pos[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = g + r * 8, tk = row / a.group;
+      const int row = g + r * 8, tk = token_of(a, row);
       pos[r] = t.pos0 + tk;
       const T *src = static_cast<const T *>(a.q) + (t.tok0 + tk) * a.q_stride + (w.head * a.group + row - tk * a.group) * D + t4 * 2;
 #pragma unroll
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int wp = 0; wp < kWarps; ++wp) sum = __fmaf_rn(sh.sum[wp][row], factor(wp, row, mx), sum);
     const bool whole = w.whole(t);
-    const int tk = row / a.group;
+    const int tk = token_of(a, row);
     float *part_o = partial_of(a, blockIdx.x, w.first ? 0 : 1, kBM, D);
     T *dst = static_cast<T *>(a.out) + (static_cast<int64_t>(t.tok0 + tk) * a.h + w.head * a.group + row - tk * a.group) * D;
     const bool none = t.pos0 + tk < 0, dead = *gave_up != 0;

@@ -253,7 +253,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t ns = 0, no = 0, nm = 0, units = 0;  // S tiles, items, masked tiles of this half; units of the CTA
     auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity, gave_up)); };
     bool ok = true;
-    for (; w.get(a, t); w.next(a)) {
+    // This half's query rows of an item into shared memory, asynchronously.
+    auto load_q = [&](const Tile &item, int head) {
+      const int n_rows = item.ntok * a.group;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const int r = (i * 128 + wt) / (D / 8), j = wt % (D / 8), qr = h * 128 + r, tk = token_of(a, qr);
+        const T *src = static_cast<const T *>(a.q) + (item.tok0 + tk) * a.q_stride + (head * a.group + qr - tk * a.group) * D + j * 8;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + h * Cfg::kTile + Cfg::chunk_at(r, j)),
+                     "l"(qr < n_rows ? src : static_cast<const T *>(a.q)), "r"(qr < n_rows ? 16 : 0)
+                     : "memory");
+      }
+    };
+    auto q_loaded = [&] {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      proxy_fence();
+      mbar_arrive(q_full + 8 * h);
+    };
+    Tile t_next;
+    bool have = w.get(a, t), q_in = false;
+    for (Walk w_next = w; have; w = w_next, t = t_next) {
+      w_next = w;
+      w_next.next(a);
+      const bool more = w_next.get(a, t_next);
+      have = more;
       const int rows = t.ntok * a.group;
       const int row = h * 128 + wt;
       const bool whole = w.whole(t);
@@ -261,23 +284,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         units += w.take;
         continue;
       }
-      const int64_t pos = t.pos0 + row / a.group;
+      const int64_t pos = t.pos0 + token_of(a, row);
       float m = -INFINITY, l = 0.f;
-      if (ok) {
-        // Q: the last item's score products are done (its last s_full was waited for).
-        unsigned char *qs = base_p + h * Cfg::kTile;
-        for (int i = wt; i < 128 * (D / 8); i += 128) {
-          const int r = i / (D / 8), j = i % (D / 8), qr = h * 128 + r;
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (qr < rows) {
-            const int tk = qr / a.group;
-            x = ld_cached(static_cast<const T *>(a.q) + (t.tok0 + tk) * a.q_stride + (w.head * a.group + qr - tk * a.group) * D + j * 8);
-          }
-          *reinterpret_cast<uint4 *>(qs + Cfg::chunk_at(r, j)) = x;
-        }
-        proxy_fence();
-        mbar_arrive(q_full + 8 * h);
+      if (ok && !q_in) {
+        load_q(t, w.head);
+        q_loaded();
       }
+      q_in = more && t_next.ntok * a.group > h * 128;  // the next item's rows are loaded behind this one's last scores
       const int64_t hi = t.pos0 + t.ntok, lo = key_lo(t, a.window);
       const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
       for (int j = 0; ok && j < w.take; ++j, ++units) {
@@ -292,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = all_wait(s_full + 8 * h, ns++ & 1);
         if (!ok) break;
         tc_fence_after();
+        if (q_in && j == w.take - 1) load_q(t_next, w_next.head);
         float s[kBN];
 #pragma unroll
         for (int i = 0; i < kBN; i += 32) tc_ld32(s_addr + i, s + i);
@@ -405,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(p_full + 8 * h);
+        if (q_in && j == w.take - 1) q_loaded();
       }
       if (ok) ok = all_wait(o_full + 8 * h, no++ & 1);
       if (!ok && wt == 0 && a.err_flag != nullptr) atomicOr(a.err_flag, XN_DEVERR_WAIT);
@@ -412,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Rows out: a thread writes its row. After a wait that gave up: NaN.
       const float nan = __int_as_float(0x7fc00000);
       float *part_o = partial_of(a, blockIdx.x, w.first ? 0 : 1, kBM, D);
-      const int tk = row / a.group;
+      const int tk = token_of(a, row);
       T *dst = static_cast<T *>(a.out) + (static_cast<int64_t>(t.tok0 + tk) * a.h + w.head * a.group + row - tk * a.group) * D;
       const float inv = __fdiv_rn(1.f, l);
 #pragma unroll
