@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kBM = kTcRows, kBN = kTcKeys, kThreads = 384;
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kPolyOf8 = 3;  // of 8 pairs of weights, those that the FMA pipe computes
 
 template <int D>
 struct TcCfg : Swizzled<D, 128> {  // a Q half, a K tile and a V tile have 128 rows
@@ -42,7 +43,6 @@ struct TcCfg : Swizzled<D, 128> {  // a Q half, a K tile and a V tile have 128 r
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -60,10 +60,26 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, float *r) {
         "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(addr));
 }
+// Loads are asynchronous: the values pass through empty statements behind the
+// wait, so that no use of them is scheduled before it.
+template <int N>
+__device__ __forceinline__ void tc_wait_ld(uint32_t *u) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; i += 4) asm volatile("" : "+r"(u[i]), "+r"(u[i + 1]), "+r"(u[i + 2]), "+r"(u[i + 3]));
+}
+__device__ __forceinline__ void tc_wait_ld(float *r) { tc_wait_ld<32>(reinterpret_cast<uint32_t *>(r)); }
 __device__ __forceinline__ void tc_ld4(uint32_t addr, uint32_t (&u)[4]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
                : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
                : "r"(addr));
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t *u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+      : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t *u) {
   asm volatile(
@@ -74,6 +90,17 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t *u) {
       "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
       "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
       : "memory");
+}
+
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
 }
 
 // D (tensor memory) = A B (+ D): A and B in shared memory, or A in tensor memory.
@@ -101,8 +128,32 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return addr >> 4 | (lbo >> 4) << 16; }
 constexpr uint32_t desc_hi(uint32_t sbo, uint32_t swizzle) { return sbo >> 4 | 1u << 14 | swizzle << 29; }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x on the FMA pipe, for the part of the weights that the exponential unit
+// has no time for (16 results a clock an SM, as many as the products leave it).
+// x = n + f, |f| <= 1/2: adding 1.5 2^23 + 127 leaves n + 127 in the low bits,
+// which shifted into place are 2^n; 2^f is a minimax polynomial (fit_exp2.py,
+// relative error 2.7e-6, against 2^-9 or 2^-12 for the rounding that follows).
+// x <= -127 gives 0, NaN stays NaN; x is at most 8 here.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  const float2 t = __fadd2_rn(x, splat2(12583039.f));
+  const float2 f = __ffma2_rn(__fadd2_rn(t, splat2(-12583039.f)), splat2(-1.f), x);
+  float2 p = __ffma2_rn(f, splat2(0x1.3997d6p-7f), splat2(0x1.ca1444p-5f));
+  p = __ffma2_rn(p, f, splat2(0x1.ec06dap-3f));
+  p = __ffma2_rn(p, f, splat2(0x1.62e0dcp-1f));
+  p = __ffma2_rn(p, f, splat2(0x1.ffffe8p-1f));
+  return __fmul2_rn(p, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
+}
+
 struct Shared {
-  uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], o_full[2], v_seen[2], drain;
+  uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2][2], o_full[2], v_seen[2], drain;
   uint32_t tmem;
   int gave_up, skip[2];
   int poison[2][3];  // non-finite values under a mask, by half; three masked tiles in turn
@@ -134,7 +185,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + 8 * i, 128);
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, 128);
+      mbar_init(p_full + 16 * i, 128);
+      mbar_init(p_full + 16 * i + 8, 128);
       mbar_init(o_full + 8 * i, 1);
       mbar_init(v_seen + 8 * i, 128);
       sh.skip[i] = sh.poison[i][0] = sh.poison[i][1] = sh.poison[i][2] = 0;
@@ -183,62 +235,94 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok)  // copies in flight end before the block does
       for (uint32_t i = n > S ? n - S : 0; i < n; ++i) wait(kv_full + 8 * (i % S), (i / S) & 1, gave_up);
    } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      constexpr uint32_t fmt = std::is_same_v<T, __half> ? 0u : 1u;
-      constexpr uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (128u >> 4) << 24;
-      constexpr uint32_t idesc_s = idesc | (kBN >> 3) << 17;
-      constexpr uint32_t idesc_o = idesc | 1u << 16 | (D >> 3) << 17;  // V: keys are the slow dimension
-      constexpr uint32_t group8 = 8 * Cfg::kRowBytes, hi = desc_hi(group8, D >= 64 ? 2 : 4);
-      uint32_t n = 0, np[2] = {0, 0}, nq[2] = {0, 0};
-      bool ok = true;
-      auto full = [&](uint32_t i) { return wait(kv_full + 8 * (i % S), (i / S) & 1, gave_up); };
-      auto scores = [&](int half, uint32_t i) {  // S[half] = Q[half] K^T, K the i-th tile loaded
-        const uint32_t q = desc_lo(base + half * Cfg::kTile, 16), k = desc_lo(kv_base + (i % S) * Cfg::kTile, 16);
+    // The whole warp walks along, and what the products need is equal in all
+    // lanes by construction (loop counters, broadcast values): their operands
+    // then sit in uniform registers. One elected lane issues. (With the walk
+    // in one lane's branch, each product took 75 clocks to issue instead of 64
+    // to run.)
+    constexpr uint32_t fmt = std::is_same_v<T, __half> ? 0u : 1u;
+    constexpr uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (128u >> 4) << 24;
+    constexpr uint32_t idesc_s = idesc | (kBN >> 3) << 17;
+    constexpr uint32_t idesc_o = idesc | 1u << 16 | (D >> 3) << 17;  // V: keys are the slow dimension
+    constexpr uint32_t group8 = 8 * Cfg::kRowBytes, hi = desc_hi(group8, D >= 64 ? 2 : 4);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    uint32_t stage = 0, phase = 0;  // of the K tile that the next scores read
+    uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
+    bool ok = true;
+    auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity, gave_up)); };
+    auto scores = [&](int half, uint32_t st) {  // S[half] = Q[half] K^T, K in stage st
+      if (elect_one()) {
+        const uint32_t q = desc_lo(base + half * Cfg::kTile, 16), k = desc_lo(kv_base + st * Cfg::kTile, 16);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk / 4 * Cfg::kSub + kk % 4 * 32) >> 4;
-          mma_ss(tmem + half * 128, q + off, k + off, hi, idesc_s, kk > 0);
+          mma_ss(tm + half * 128, q + off, k + off, hi, idesc_s, kk > 0);
         }
         tc_commit(s_full + 8 * half);
-      };
-      auto output = [&](int half, uint32_t i, bool add) {  // O[half] (+)= P[half] V, V the i-th tile loaded
-        const uint32_t v = desc_lo(kv_base + (i % S) * Cfg::kTile, Cfg::kSub);
+      }
+      __syncwarp();
+    };
+    auto output = [&](int half, int keys, uint32_t st, bool add) {  // O[half] (+)= P[half] V over 64 keys, V in stage st
+      if (elect_one()) {
+        const uint32_t v = desc_lo(kv_base + st * Cfg::kTile, Cfg::kSub);
 #pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk)
-          mma_ts(tmem + o_col + half * D, tmem + half * 128 + kk * 8, v + (kk * 2 * group8 >> 4), hi, idesc_o, add || kk > 0);
-      };
-      for (; ok && w.get(a, t); w.next(a)) {
-        const int halves = t.ntok * a.group > 128 ? 2 : 1;
-        ok = full(n);
-        for (int h = 0; ok && h < halves; ++h) {
-          ok = wait(q_full + 8 * h, nq[h]++ & 1, gave_up);
+        for (int kk = keys * 4; kk < keys * 4 + 4; ++kk)
+          mma_ts(tm + o_col + half * D, tm + half * 128 + kk * 8, v + (kk * 2 * group8 >> 4), hi, idesc_o, add || kk > 0);
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint32_t bar) {
+      if (elect_one()) tc_commit(bar);
+      __syncwarp();
+    };
+    auto advance = [&](uint32_t &st, uint32_t &ph) {
+      if (++st == S) {
+        st = 0;
+        ph ^= 1;
+      }
+    };
+    for (; ok && w.get(a, t); w.next(a)) {
+      const int halves = __shfl_sync(0xffffffffu, t.ntok * a.group > 128 ? 2 : 1, 0);
+      const int take = __shfl_sync(0xffffffffu, w.take, 0);
+      ok = all_wait(kv_full + 8 * stage, phase);
+      for (int h = 0; ok && h < halves; ++h) {
+        ok = all_wait(q_full + 8 * h, nq[h]++ & 1);
+        if (!ok) break;
+        tc_fence_after();
+        scores(h, stage);
+      }
+      if (!ok) break;
+      commit(kv_empty + 8 * stage);
+      for (int j = 0; ok && j < take; ++j) {
+        const bool more = j + 1 < take;
+        advance(stage, phase);
+        const uint32_t v_st = stage, v_ph = phase;
+        advance(stage, phase);  // the next K, of this item or the next one
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == halves) break;
+          ok = all_wait(p_full + 16 * h, np[h] & 1);
+          if (ok && h == 0) ok = all_wait(kv_full + 8 * v_st, v_ph) && (!more || all_wait(kv_full + 8 * stage, phase));
           if (!ok) break;
           tc_fence_after();
-          scores(h, n);
+          const bool skip = __shfl_sync(0xffffffffu, *static_cast<volatile int *>(&sh.skip[h]), 0) != 0;
+          if (!skip) output(h, 0, v_st, j > 0);
+          ok = all_wait(p_full + 16 * h + 8, np[h]++ & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (!skip) output(h, 1, v_st, true);
+          if (h == halves - 1) commit(kv_empty + 8 * v_st);
+          if (more)
+            scores(h, stage);
+          else
+            commit(o_full + 8 * h);
         }
-        if (!ok) break;
-        tc_commit(kv_empty + 8 * (n % S));
-        for (int j = 0; ok && j < w.take; ++j) {
-          const bool more = j + 1 < w.take;
-          for (int h = 0; h < halves; ++h) {
-            ok = wait(p_full + 8 * h, np[h]++ & 1, gave_up) && (h > 0 || (full(n + 1) && (!more || full(n + 2))));
-            if (!ok) break;
-            tc_fence_after();
-            if (!*static_cast<volatile int *>(&sh.skip[h])) output(h, n + 1, j > 0);
-            if (h == halves - 1) tc_commit(kv_empty + 8 * ((n + 1) % S));
-            if (more)
-              scores(h, n + 2);
-            else
-              tc_commit(o_full + 8 * h);
-          }
-          if (ok && more) tc_commit(kv_empty + 8 * ((n + 2) % S));
-          n += 2;
-        }
+        if (ok && more) commit(kv_empty + 8 * stage);
       }
-      if (!ok) {  // products in flight end before tensor memory is freed
-        tc_commit(smem_u32(&sh.drain));
-        for (int i = 0; i < 1 << 20 && !mbar_try(smem_u32(&sh.drain), 0); ++i) {
-        }
+    }
+    if (!ok) {  // products in flight end before tensor memory is freed
+      commit(smem_u32(&sh.drain));
+      for (int i = 0; i < 1 << 20 && !mbar_try(smem_u32(&sh.drain), 0); ++i) {
       }
     }
     __syncwarp();
@@ -292,16 +376,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       q_in = more && t_next.ntok * a.group > h * 128;  // the next item's rows are loaded behind this one's last scores
       const int64_t hi = t.pos0 + t.ntok, lo = key_lo(t, a.window);
-      const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
+      const int64_t u0 = first_unit(t, a.window, kBN) + w.k, key0 = u0 * kBN;
+      // Of this segment's key tiles those from j_diag on hold keys behind the first token, those up to j_win
+      // keys before the last token's window: some row does not see them.
+      const int j_diag = static_cast<int>((t.pos0 < 0 ? 0 : (t.pos0 + 1) / kBN) - u0);
+      const int j_win = a.window > 0 && hi - 1 >= a.window ? static_cast<int>((hi - 1 - a.window) / kBN - u0) : -1;
+      const int64_t row_lo = a.window > 0 && pos - a.window + 1 > key0 ? pos - a.window + 1 - key0 : 0;
+      const int see_lo = static_cast<int>(row_lo < (1 << 30) ? row_lo : 1 << 30), see_hi = static_cast<int>(pos + 1 - key0);
       for (int j = 0; ok && j < w.take; ++j, ++units) {
-        const int64_t key0 = (u0 + j) * kBN;
-        const bool masked = key0 + kBN - 1 > t.pos0 || (a.window > 0 && key0 <= hi - 1 - a.window);
-        int seen_lo = 0, seen_hi = kBN;  // keys of the tile that this row sees
-        if (masked) {
-          const int64_t e = pos + 1 - key0, b = a.window > 0 ? e - a.window : 0;
-          seen_hi = static_cast<int>(e < 0 ? 0 : e > kBN ? kBN : e);
-          seen_lo = static_cast<int>(b < 0 ? 0 : b > kBN ? kBN : b);
-        }
+        const bool masked = j >= j_diag || j <= j_win;
+        const int seen_lo = see_lo - j * kBN, seen_hi = see_hi - j * kBN;  // keys of the tile that this row sees, if masked
         ok = all_wait(s_full + 8 * h, ns++ & 1);
         if (!ok) break;
         tc_fence_after();
@@ -309,15 +393,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         float s[kBN];
 #pragma unroll
         for (int i = 0; i < kBN; i += 32) tc_ld32(s_addr + i, s + i);
-        tc_wait_ld();
+        tc_wait_ld<kBN>(reinterpret_cast<uint32_t *>(s));
         if (masked) {
 #pragma unroll
           for (int i = 0; i < kBN; ++i) s[i] = i >= seen_lo && i < seen_hi ? s[i] : -INFINITY;
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < kBN; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int i = 4; i + 8 <= kBN; i += 8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + 2 * k], s[i + 2 * k + 1]);
+        }
+        const float top = max3(max3(mx[0], s[kBN - 4], s[kBN - 3]), max3(mx[1], s[kBN - 2], s[kBN - 1]), fmaxf(mx[2], mx[3]));
         // A larger maximum by more than 2^8: this warp's rows move to it.
         if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
           const float to = fmaxf(m, top), f = m == to ? 1.f : ex2_approx_ftz((m - to) * c);
@@ -328,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < D; i += 32) {
               float o[32];
               tc_ld32(o_addr + i, o);
-              tc_wait_ld();
+              tc_wait_ld(o);
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] *= f;
               tc_st32(o_addr + i, reinterpret_cast<uint32_t *>(o));
@@ -336,25 +423,37 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float mc = m == -INFINITY ? 0.f : -m * c;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t p[kBN / 2];
+        float2 sum[2] = {splat2(0.f), splat2(0.f)};
 #pragma unroll
-        for (int i = 0; i < kBN; i += 2) {
-          const float x = ex2_approx_ftz(__fmaf_rn(s[i], c, mc)), y = ex2_approx_ftz(__fmaf_rn(s[i + 1], c, mc));
-          sum[i & 3] += x;
-          sum[(i + 1) & 3] += y;
-          p[i / 2] = pack2<T>(x, y);
+        for (int i = 0; i < 4; ++i) {
+          const float *x = s + i * 32;
+          uint32_t p[16];  // in place of the scores
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float2 e = __ffma2_rn(make_float2(x[2 * k], x[2 * k + 1]), splat2(c), splat2(mc));
+            if (k % 8 >= 8 - kPolyOf8)
+              e = exp2_poly(e);
+            else
+              e = make_float2(ex2_approx_ftz(e.x), ex2_approx_ftz(e.y));
+            sum[k & 1] = __fadd2_rn(sum[k & 1], e);
+            p[k] = pack2<T>(e.x, e.y);
+          }
+          tc_st16(s_addr + 16 * i, p);
+          if (i == 1 && !masked) {  // the product over the first 64 keys may begin
+            if (wt == 0) *static_cast<volatile int *>(&sh.skip[h]) = 0;
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(p_full + 16 * h);
+          }
         }
-        tc_st32(s_addr, p);
-        tc_st32(s_addr + 32, p + 32);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
         int poisoned = 0;
         if (masked) {
           const uint32_t nv = 2 * units + 1;
           ok = all_wait(kv_full + 8 * (nv % S), (nv / S) & 1);
           if (!ok) break;
           unsigned char *vs = base_p + 2 * Cfg::kTile + (nv % S) * Cfg::kTile;
-          const int64_t key = key0 + wt;  // this thread's V row
+          const int64_t key = key0 + j * kBN + wt;  // this thread's V row
           bool bad = false;
           if (key >= hi || key < lo) {
             for (int q = 0; q < D / 8; ++q) *reinterpret_cast<uint4 *>(vs + Cfg::chunk_at(wt, q)) = make_uint4(0u, 0u, 0u, 0u);
@@ -381,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               float o[32];
               if (j > 0) {
                 tc_ld32(o_addr + i, o);
-                tc_wait_ld();
+                tc_wait_ld(o);
               } else {
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] = 0.f;
@@ -391,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t pw[4];
                 __syncwarp();
                 tc_ld4(s_addr + kb / 2, pw);
-                tc_wait_ld();
+                tc_wait_ld<4>(pw);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                   if (kb + k < seen_lo || kb + k >= seen_hi) continue;
@@ -415,10 +514,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (wt == 0) *static_cast<volatile int *>(&sh.skip[h]) = poisoned;
+        if (masked && wt == 0) *static_cast<volatile int *>(&sh.skip[h]) = poisoned;
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(p_full + 8 * h);
+        if (masked) mbar_arrive(p_full + 16 * h);
+        mbar_arrive(p_full + 16 * h + 8);
         if (q_in && j == w.take - 1) q_loaded();
       }
       if (ok) ok = all_wait(o_full + 8 * h, no++ & 1);
@@ -436,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (ok) {
           tc_ld32(o_addr + i, o);
-          tc_wait_ld();
+          tc_wait_ld(o);
         } else {
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = nan;
