@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       int page = ld.page(a, t, u0 * kBN, lo, hi);
       for (int64_t u = u0; u < u0 + w.take; ++u, ++n) {
         const uint32_t st = n % S, round = n / S;
-        ok = __all_sync(0xffffffffu, round == 0 || wait(empty + 8 * st, (round - 1) & 1, gave_up));
+        ok = round == 0 || wait(empty + 8 * st, (round - 1) & 1, gave_up);
         if (!ok) break;
         if (lane == 0) mbar_expect(full + 8 * st, 2 * Cfg::kTile);
         __syncwarp();
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
     for (int64_t u = u0; u < u0 + w.take; ++u, ++n) {
       const uint32_t st = n % S;
-      ok = ok && __all_sync(0xffffffffu, wait(full + 8 * st, (n / S) & 1, gave_up));
+      ok = ok && wait(full + 8 * st, (n / S) & 1, gave_up);
       if (!ok) continue;
       const uint32_t ks = base + st * 2 * Cfg::kTile, vs = ks + Cfg::kTile;
       float s[2][4] = {};
@@ -240,8 +240,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + 8 * st);
+      warp_arrive(empty + 8 * st);
     }
     // The warps' parts come together, 32 columns at a time.
 #pragma unroll

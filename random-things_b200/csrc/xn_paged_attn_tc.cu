@@ -31,7 +31,7 @@ namespace paged {
 namespace {
 
 constexpr int kBM = kTcRows, kBN = kTcKeys, kThreads = 384;
-constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;  // and 10: one for each half
 constexpr int kPolyOf8 = 3;  // of 8 pairs of weights, those that the FMA pipe computes
 
 template <int D>
@@ -152,8 +152,17 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   return __fmul2_rn(p, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 
+// Of a segment's key tiles, the first of them number u0, those from j_diag on
+// hold keys behind the first token, those up to j_win keys before the last
+// token's window: some row does not see them.
+__device__ __forceinline__ void masked_tiles(const Args &a, const Tile &t, int64_t u0, int &j_diag, int &j_win) {
+  const int64_t last = t.pos0 + t.ntok - 1;
+  j_diag = static_cast<int>((t.pos0 < 0 ? 0 : (t.pos0 + 1) / kBN) - u0);
+  j_win = a.window > 0 && last >= a.window ? static_cast<int>((last - a.window) / kBN - u0) : -1;
+}
+
 struct Shared {
-  uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2][2], o_full[2], v_seen[2], drain;
+  uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], o_full[2], v_seen[2], drain[2];
   uint32_t tmem;
   int gave_up, skip[2];
   int poison[2][3];  // non-finite values under a mask, by half; three masked tiles in turn
@@ -180,18 +189,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(kv_full + 8 * i, 1);
-      mbar_init(kv_empty + 8 * i, 1);
+      mbar_init(kv_empty + 8 * i, 2);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + 8 * i, 128);
+      mbar_init(q_full + 8 * i, 4);
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 16 * i, 128);
-      mbar_init(p_full + 16 * i + 8, 128);
+      mbar_init(p_full + 8 * i, 4);
       mbar_init(o_full + 8 * i, 1);
-      mbar_init(v_seen + 8 * i, 128);
+      mbar_init(v_seen + 8 * i, 4);
       sh.skip[i] = sh.poison[i][0] = sh.poison[i][1] = sh.poison[i][2] = 0;
     }
-    mbar_init(smem_u32(&sh.drain), 1);
+    mbar_init(smem_u32(&sh.drain[0]), 1);
+    mbar_init(smem_u32(&sh.drain[1]), 1);
     sh.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     proxy_fence();
@@ -224,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++n) {
           const uint32_t st = n % S, round = n / S;
-          ok = __all_sync(0xffffffffu, round == 0 || wait(kv_empty + 8 * st, (round - 1) & 1, gave_up));
+          ok = round == 0 || wait(kv_empty + 8 * st, (round - 1) & 1, gave_up);
           if (!ok) break;
           if (lane == 0) mbar_expect(kv_full + 8 * st, Cfg::kTile);
           __syncwarp();
@@ -234,40 +243,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok)  // copies in flight end before the block does
       for (uint32_t i = n > S ? n - S : 0; i < n; ++i) wait(kv_full + 8 * (i % S), (i / S) & 1, gave_up);
-   } else if (warp == kMmaWarp) {
-    // The whole warp walks along, and what the products need is equal in all
-    // lanes by construction (loop counters, broadcast values): their operands
-    // then sit in uniform registers. One elected lane issues. (With the walk
-    // in one lane's branch, each product took 75 clocks to issue instead of 64
-    // to run.)
+   } else if (warp < kMmaWarp + 2) {
+    // A warp for each half, so that what one waits for does not hold up the other. The whole warp walks along, and
+    // what the products need is equal in all lanes by construction (loop counters, broadcast values): their operands
+    // then sit in uniform registers. One elected lane issues. (With the walk in one lane's branch, each product took
+    // 75 clocks to issue instead of 64 to run.)
     constexpr uint32_t fmt = std::is_same_v<T, __half> ? 0u : 1u;
     constexpr uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (128u >> 4) << 24;
     constexpr uint32_t idesc_s = idesc | (kBN >> 3) << 17;
     constexpr uint32_t idesc_o = idesc | 1u << 16 | (D >> 3) << 17;  // V: keys are the slow dimension
     constexpr uint32_t group8 = 8 * Cfg::kRowBytes, hi = desc_hi(group8, D >= 64 ? 2 : 4);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int h = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), s_col = tm + h * 128, o_at = tm + o_col + h * D;
+    const uint32_t q_desc = desc_lo(base + h * Cfg::kTile, 16);
     uint32_t stage = 0, phase = 0;  // of the K tile that the next scores read
-    uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
+    uint32_t np = 0, nq = 0;
     bool ok = true;
-    auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity, gave_up)); };
-    auto scores = [&](int half, uint32_t st) {  // S[half] = Q[half] K^T, K in stage st
+    auto scores = [&](uint32_t st) {  // S = Q K^T, K in stage st
       if (elect_one()) {
-        const uint32_t q = desc_lo(base + half * Cfg::kTile, 16), k = desc_lo(kv_base + st * Cfg::kTile, 16);
+        const uint32_t k = desc_lo(kv_base + st * Cfg::kTile, 16);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk / 4 * Cfg::kSub + kk % 4 * 32) >> 4;
-          mma_ss(tm + half * 128, q + off, k + off, hi, idesc_s, kk > 0);
+          mma_ss(s_col, q_desc + off, k + off, hi, idesc_s, kk > 0);
         }
-        tc_commit(s_full + 8 * half);
+        tc_commit(s_full + 8 * h);
+        tc_commit(kv_empty + 8 * st);
       }
       __syncwarp();
     };
-    auto output = [&](int half, int keys, uint32_t st, bool add) {  // O[half] (+)= P[half] V over 64 keys, V in stage st
+    auto output = [&](uint32_t st, bool add) {  // O (+)= P V, V in stage st
       if (elect_one()) {
         const uint32_t v = desc_lo(kv_base + st * Cfg::kTile, Cfg::kSub);
 #pragma unroll
-        for (int kk = keys * 4; kk < keys * 4 + 4; ++kk)
-          mma_ts(tm + o_col + half * D, tm + half * 128 + kk * 8, v + (kk * 2 * group8 >> 4), hi, idesc_o, add || kk > 0);
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          mma_ts(o_at, s_col + kk * 8, v + (kk * 2 * group8 >> 4), hi, idesc_o, add || kk > 0);
+        tc_commit(kv_empty + 8 * st);
       }
       __syncwarp();
     };
@@ -275,57 +286,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) tc_commit(bar);
       __syncwarp();
     };
-    auto advance = [&](uint32_t &st, uint32_t &ph) {
-      if (++st == S) {
-        st = 0;
-        ph ^= 1;
+    auto advance = [&] {
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1;
       }
     };
     for (; ok && w.get(a, t); w.next(a)) {
-      const int halves = __shfl_sync(0xffffffffu, t.ntok * a.group > 128 ? 2 : 1, 0);
       const int take = __shfl_sync(0xffffffffu, w.take, 0);
-      ok = all_wait(kv_full + 8 * stage, phase);
-      for (int h = 0; ok && h < halves; ++h) {
-        ok = all_wait(q_full + 8 * h, nq[h]++ & 1);
+      if (__shfl_sync(0xffffffffu, t.ntok * a.group <= h * 128 ? 1 : 0, 0)) {
+        // Nothing to do for this half, but the stages wait for its word too.
+        for (int i = 0; ok && i < 2 * take; ++i) {
+          ok = wait(kv_full + 8 * stage, phase, gave_up);
+          if (ok && lane == 0) mbar_arrive(kv_empty + 8 * stage);
+          advance();
+        }
+        continue;
+      }
+      // Key tiles with a mask: only there a poisoned tile can be (see the softmax).
+      int j_diag, j_win;
+      masked_tiles(a, t, first_unit(t, a.window, kBN) + w.k, j_diag, j_win);
+      j_diag = __shfl_sync(0xffffffffu, j_diag, 0);
+      j_win = __shfl_sync(0xffffffffu, j_win, 0);
+      ok = wait(kv_full + 8 * stage, phase, gave_up) && wait(q_full + 8 * h, nq++ & 1, gave_up);
+      if (!ok) break;
+      tc_fence_after();
+      scores(stage);
+      for (int j = 0; j < take; ++j) {
+        const bool more = j + 1 < take;
+        advance();
+        const uint32_t v_st = stage;
+        ok = wait(kv_full + 8 * stage, phase, gave_up);
+        advance();  // the next K, of this item or the next one
+        if (ok && more) ok = wait(kv_full + 8 * stage, phase, gave_up);
+        if (ok) ok = wait(p_full + 8 * h, np++ & 1, gave_up);
         if (!ok) break;
         tc_fence_after();
-        scores(h, stage);
-      }
-      if (!ok) break;
-      commit(kv_empty + 8 * stage);
-      for (int j = 0; ok && j < take; ++j) {
-        const bool more = j + 1 < take;
-        advance(stage, phase);
-        const uint32_t v_st = stage, v_ph = phase;
-        advance(stage, phase);  // the next K, of this item or the next one
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h == halves) break;
-          ok = all_wait(p_full + 16 * h, np[h] & 1);
-          if (ok && h == 0) ok = all_wait(kv_full + 8 * v_st, v_ph) && (!more || all_wait(kv_full + 8 * stage, phase));
-          if (!ok) break;
-          tc_fence_after();
-          const bool skip = __shfl_sync(0xffffffffu, *static_cast<volatile int *>(&sh.skip[h]), 0) != 0;
-          if (!skip) output(h, 0, v_st, j > 0);
-          ok = all_wait(p_full + 16 * h + 8, np[h]++ & 1);
-          if (!ok) break;
-          tc_fence_after();
-          if (!skip) output(h, 1, v_st, true);
-          if (h == halves - 1) commit(kv_empty + 8 * v_st);
-          if (more)
-            scores(h, stage);
-          else
-            commit(o_full + 8 * h);
-        }
-        if (ok && more) commit(kv_empty + 8 * stage);
+        int skip = 0;
+        if (j >= j_diag || j <= j_win) skip = __shfl_sync(0xffffffffu, *static_cast<volatile int *>(&sh.skip[h]), 0);
+        if (!skip)
+          output(v_st, j > 0);
+        else
+          commit(kv_empty + 8 * v_st);
+        if (more)
+          scores(stage);
+        else
+          commit(o_full + 8 * h);
       }
     }
     if (!ok) {  // products in flight end before tensor memory is freed
-      commit(smem_u32(&sh.drain));
-      for (int i = 0; i < 1 << 20 && !mbar_try(smem_u32(&sh.drain), 0); ++i) {
+      commit(smem_u32(&sh.drain[h]));
+      for (int i = 0; i < 1 << 20 && !mbar_try(smem_u32(&sh.drain[h]), 0); ++i) {
       }
     }
-    __syncwarp();
    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -335,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + lanes + h * 128, o_addr = tmem + lanes + o_col + h * D;
     const float c = a.scale_log2;
     uint32_t ns = 0, no = 0, nm = 0, units = 0;  // S tiles, items, masked tiles of this half; units of the CTA
-    auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity, gave_up)); };
+    auto all_wait = [&](uint32_t bar, uint32_t parity) { return wait(bar, parity, gave_up); };
     bool ok = true;
     // This half's query rows of an item into shared memory, asynchronously.
     auto load_q = [&](const Tile &item, int head) {
@@ -352,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto q_loaded = [&] {
       asm volatile("cp.async.wait_all;" ::: "memory");
       proxy_fence();
-      mbar_arrive(q_full + 8 * h);
+      warp_arrive(q_full + 8 * h);
     };
     Tile t_next;
     bool have = w.get(a, t), q_in = false;
@@ -377,10 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       q_in = more && t_next.ntok * a.group > h * 128;  // the next item's rows are loaded behind this one's last scores
       const int64_t hi = t.pos0 + t.ntok, lo = key_lo(t, a.window);
       const int64_t u0 = first_unit(t, a.window, kBN) + w.k, key0 = u0 * kBN;
-      // Of this segment's key tiles those from j_diag on hold keys behind the first token, those up to j_win
-      // keys before the last token's window: some row does not see them.
-      const int j_diag = static_cast<int>((t.pos0 < 0 ? 0 : (t.pos0 + 1) / kBN) - u0);
-      const int j_win = a.window > 0 && hi - 1 >= a.window ? static_cast<int>((hi - 1 - a.window) / kBN - u0) : -1;
+      int j_diag, j_win;
+      masked_tiles(a, t, u0, j_diag, j_win);
       const int64_t row_lo = a.window > 0 && pos - a.window + 1 > key0 ? pos - a.window + 1 - key0 : 0;
       const int see_lo = static_cast<int>(row_lo < (1 << 30) ? row_lo : 1 << 30), see_hi = static_cast<int>(pos + 1 - key0);
       for (int j = 0; ok && j < w.take; ++j, ++units) {
@@ -439,12 +450,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             p[k] = pack2<T>(e.x, e.y);
           }
           tc_st16(s_addr + 16 * i, p);
-          if (i == 1 && !masked) {  // the product over the first 64 keys may begin
-            if (wt == 0) *static_cast<volatile int *>(&sh.skip[h]) = 0;
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(p_full + 16 * h);
-          }
         }
         l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
         int poisoned = 0;
@@ -469,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           volatile int *poison = sh.poison[h];
           if (bad) poison[nm % 3] = 1;
           if (wt == 0) poison[(nm + 1) % 3] = 0;
-          mbar_arrive(v_seen + 8 * h);
+          warp_arrive(v_seen + 8 * h);
           ok = all_wait(v_seen + 8 * h, nm & 1);
           if (!ok) break;
           poisoned = poison[nm++ % 3];
@@ -517,8 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (masked && wt == 0) *static_cast<volatile int *>(&sh.skip[h]) = poisoned;
         tc_wait_st();
         tc_fence_before();
-        if (masked) mbar_arrive(p_full + 16 * h);
-        mbar_arrive(p_full + 16 * h + 8);
+        warp_arrive(p_full + 8 * h);
         if (q_in && j == w.take - 1) q_loaded();
       }
       if (ok) ok = all_wait(o_full + 8 * h, no++ & 1);

@@ -12,7 +12,7 @@ namespace xn {
 namespace paged {
 namespace {
 
-constexpr uint64_t kWaitNs = 2000000000ull;  // a wait gives up after 2 s
+constexpr long long kWaitClocks = 4000000000ll;  // a wait gives up after 2 s or more
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -37,21 +37,28 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Waits for the phase of `parity`; false when it did not come within kWaitNs or
-// another role gave up (then nothing that the phase stands for may be used).
+// Waits with a converged warp for the phase of `parity`; false when it did not
+// come within kWaitClocks or another role gave up (then nothing that the phase
+// stands for may be used). All lanes poll: with one lane polling in a branch of
+// its own, what follows no longer counts as equal in all lanes, and operands
+// leave the uniform registers (measured: prefill of 8192 tokens 0.69 -> 0.89 ms).
 // Inlined: with a call in the kernel its register split would not take effect.
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
-  uint64_t t0 = 0, t;
-  while (true) {
+  bool got = mbar_try(bar, parity);
+  if (!got) {
+    const long long t0 = clock64();
+    do {
 #pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try(bar, parity)) return true;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t0 == 0) t0 = t;
-    if (*gave_up || t - t0 > kWaitNs) break;
+      for (int i = 0; i < 64 && !got; ++i) got = mbar_try(bar, parity);
+    } while (!got && !*gave_up && clock64() - t0 < kWaitClocks);
+    if (!got) *gave_up = 1;
   }
-  *gave_up = 1;
-  return false;
+  return __all_sync(0xffffffffu, got);
+}
+// One arrival for a warp, behind what all its lanes did.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
