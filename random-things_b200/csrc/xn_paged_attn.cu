@@ -344,7 +344,7 @@ struct Shape {
 Shape shape_of(int64_t group, int64_t max_new, int dtype) {
   const bool few = max_new * group <= 16 && group <= 16;
   if (dtype == XN_F32) return Shape{few ? 16 : 64, 64, 2 * sm_count(), 1, 4};
-  return few ? Shape{kDecRows, kDecKeys, 2 * sm_count(), 2, 6} : Shape{kTcRows, kTcKeys, sm_count(), 3, 5};
+  return few ? Shape{kDecRows, kDecKeys, 2 * sm_count(), 2, 6} : Shape{kTcRows, kTcKeys, sm_count(), 6, 10};
 }
 
 struct Layout {

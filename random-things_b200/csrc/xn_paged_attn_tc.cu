@@ -2,14 +2,16 @@
 // tokens on the 5th-generation tensor cores (sm_100a).
 //
 // A CTA takes 256 rows (token, query head of the group) of one kv head: two
-// halves of 128, each with its own softmax warpgroup, scores S and output O in
-// tensor memory. Per key tile of 128 keys:
+// halves of 128, each with its own softmax warpgroup, product warp, scores S
+// (two buffers) and output O in tensor memory. Per key tile of 64 keys:
 //   S = Q K^T      tcgen05.mma, both operands in shared memory
 //   P = exp2(S c - m c), row maxima and sums   one thread a row: no shuffles
 //   O = O + P V    tcgen05.mma, P in tensor memory (over S), V in shared memory
-// While one half's softmax runs, the tensor cores work for the other half.
-// One warp loads: K and V tiles come by TMA, a box per page, swizzled as the
-// MMA reads them, through a ring of stages; another warp issues the MMAs.
+// The scores of the next two tiles are issued ahead, so that a half's softmax
+// need not wait for its own products. (With one buffer of 128 keys each half
+// went softmax, products, softmax, ...: 4600 clocks for 256 x 128 against 2048
+// of the products alone.) One more warp loads: K and V tiles come by TMA, a box
+// per page, swizzled as the MMA reads them, through two rings of stages.
 //
 // O stays in tensor memory for all key tiles. When a row's maximum grows by
 // more than 2^8 (in the exponent's units: 8), its warp rescales O; below that
@@ -32,13 +34,14 @@ namespace {
 
 constexpr int kBM = kTcRows, kBN = kTcKeys, kThreads = 384;
 constexpr int kLoadWarp = 8, kMmaWarp = 9;  // and 10: one for each half
-constexpr int kPolyOf8 = 3;  // of 8 pairs of weights, those that the FMA pipe computes
+constexpr int kPolyOf8 = 2;  // of 8 pairs of weights, those that the FMA pipe computes
 
 template <int D>
-struct TcCfg : Swizzled<D, 128> {  // a Q half, a K tile and a V tile have 128 rows
-  using Swizzled<D, 128>::kTile;
-  static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr size_t kSmem = 1024 + 2 * kTile + kStages * kTile;
+struct TcCfg {
+  using Q = Swizzled<D, 128>;  // a half's query rows
+  using KV = Swizzled<D, kBN>;  // a K or V tile
+  static constexpr int kStages = D == 128 ? 5 : 8;  // of each ring
+  static constexpr size_t kSmem = 1024 + 2 * Q::kTile + 2 * kStages * KV::kTile;
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -73,13 +76,6 @@ __device__ __forceinline__ void tc_ld4(uint32_t addr, uint32_t (&u)[4]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
                : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
                : "r"(addr));
-}
-__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t *u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
-      : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t *u) {
   asm volatile(
@@ -162,9 +158,10 @@ __device__ __forceinline__ void masked_tiles(const Args &a, const Tile &t, int64
 }
 
 struct Shared {
-  uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], o_full[2], v_seen[2], drain[2];
+  uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], v_seen[2], drain[2];  // [half][S buffer]
   uint32_t tmem;
-  int gave_up, skip[2];
+  int gave_up, skip[2][2];  // skip: a poisoned tile's product is done already
   int poison[2][3];  // non-finite values under a mask, by half; three masked tiles in turn
 };
 
@@ -174,33 +171,38 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_wait();
   griddep_release();
   using Cfg = TcCfg<D>;
+  using Q = typename Cfg::Q;
+  using KV = typename Cfg::KV;
   constexpr int S = Cfg::kStages;
   extern __shared__ unsigned char tc_smem[];
   __shared__ Shared sh;
   const uint32_t base = (smem_u32(tc_smem) + 1023u) & ~1023u;
   unsigned char *base_p = tc_smem + (base - smem_u32(tc_smem));
-  const uint32_t kv_base = base + 2 * Cfg::kTile;
+  const uint32_t k_base = base + 2 * Q::kTile, v_base = k_base + S * KV::kTile;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int *gave_up = &sh.gave_up;
 
-  const uint32_t kv_full = smem_u32(sh.kv_full), kv_empty = smem_u32(sh.kv_empty), q_full = smem_u32(sh.q_full);
-  const uint32_t s_full = smem_u32(sh.s_full), p_full = smem_u32(sh.p_full), o_full = smem_u32(sh.o_full);
-  const uint32_t v_seen = smem_u32(sh.v_seen);
+  const uint32_t k_full = smem_u32(sh.k_full), k_empty = smem_u32(sh.k_empty), v_full = smem_u32(sh.v_full);
+  const uint32_t v_empty = smem_u32(sh.v_empty), q_full = smem_u32(sh.q_full), s_full = smem_u32(sh.s_full);
+  const uint32_t p_full = smem_u32(sh.p_full), pv_done = smem_u32(sh.pv_done), v_seen = smem_u32(sh.v_seen);
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(kv_full + 8 * i, 1);
-      mbar_init(kv_empty + 8 * i, 2);
+      mbar_init(k_full + 8 * i, 1);
+      mbar_init(k_empty + 8 * i, 2);
+      mbar_init(v_full + 8 * i, 1);
+      mbar_init(v_empty + 8 * i, 2);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + 8 * i, 4);
-      mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, 4);
-      mbar_init(o_full + 8 * i, 1);
-      mbar_init(v_seen + 8 * i, 4);
-      sh.skip[i] = sh.poison[i][0] = sh.poison[i][1] = sh.poison[i][2] = 0;
+      mbar_init(q_full + 8 * i, 128);
+      mbar_init(v_seen + 8 * i, 128);
+      mbar_init(smem_u32(&sh.drain[i]), 1);
+      sh.skip[i][0] = sh.skip[i][1] = sh.poison[i][0] = sh.poison[i][1] = sh.poison[i][2] = 0;
     }
-    mbar_init(smem_u32(&sh.drain[0]), 1);
-    mbar_init(smem_u32(&sh.drain[1]), 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 128);
+      mbar_init(pv_done + 8 * i, 1);
+    }
     sh.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     proxy_fence();
@@ -213,37 +215,43 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  // Tensor memory: S of the halves at columns 0 and 128 (P over them), O behind.
+  // Tensor memory: two S buffers a half at columns 0 .. 255 (P over them), O behind.
   const uint32_t o_col = 256;
 
-  // 384 x 168 registers at launch, split as 2 x 128 x 208 + 128 x 88.
   Tile t;
-  if (warp >= kLoadWarp) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-   Walk w(a, blockIdx.x);
-   if (warp == kLoadWarp) {
+  Walk w(a, blockIdx.x);
+  if (warp == kLoadWarp) {
     const TileLoad<D, kBN> ld(a);
-    uint32_t n = 0;  // tiles loaded
+    uint32_t nk = 0, nv = 0;  // tiles loaded
     bool ok = true;
+    auto load = [&](const CUtensorMap *map, uint32_t ring, uint32_t full, uint32_t empty, uint32_t &n, int64_t key0, int page) {
+      const uint32_t st = n % S, round = n / S;
+      ok = ok && (round == 0 || wait(empty + 8 * st, (round - 1) & 1, gave_up));
+      if (!ok) return;
+      if (lane == 0) mbar_expect(full + 8 * st, KV::kTile);
+      __syncwarp();
+      ld.load(a, map, ring + st * KV::kTile, full + 8 * st, key0, w.head, page);
+      ++n;
+    };
     for (; ok && w.get(a, t); w.next(a)) {
       const int64_t hi = t.pos0 + t.ntok, lo = key_lo(t, a.window);
       const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
-      for (int64_t u = u0; ok && u < u0 + w.take; ++u) {
-        const int page = ld.page(a, t, u * kBN, lo, hi);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++n) {
-          const uint32_t st = n % S, round = n / S;
-          ok = round == 0 || wait(kv_empty + 8 * st, (round - 1) & 1, gave_up);
-          if (!ok) break;
-          if (lane == 0) mbar_expect(kv_full + 8 * st, Cfg::kTile);
-          __syncwarp();
-          ld.load(a, kv ? &vmap : &kmap, kv_base + st * Cfg::kTile, kv_full + 8 * st, u * kBN, w.head, page);
-        }
+      // In the order of use: K runs one tile ahead of V.
+      int v_page = 0;
+      for (int j = 0; ok && j < w.take; ++j) {
+        const int64_t key0 = (u0 + j) * kBN;
+        const int page = ld.page(a, t, key0, lo, hi);
+        load(&kmap, k_base, k_full, k_empty, nk, key0, page);
+        if (j > 0) load(&vmap, v_base, v_full, v_empty, nv, key0 - kBN, v_page);
+        v_page = page;
       }
+      load(&vmap, v_base, v_full, v_empty, nv, (u0 + w.take - 1) * kBN, v_page);
     }
-    if (!ok)  // copies in flight end before the block does
-      for (uint32_t i = n > S ? n - S : 0; i < n; ++i) wait(kv_full + 8 * (i % S), (i / S) & 1, gave_up);
-   } else if (warp < kMmaWarp + 2) {
+    if (!ok) {  // copies in flight end before the block does
+      for (uint32_t i = nk > S ? nk - S : 0; i < nk; ++i) wait(k_full + 8 * (i % S), (i / S) & 1, gave_up);
+      for (uint32_t i = nv > S ? nv - S : 0; i < nv; ++i) wait(v_full + 8 * (i % S), (i / S) & 1, gave_up);
+    }
+  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     // A warp for each half, so that what one waits for does not hold up the other. The whole warp walks along, and
     // what the products need is equal in all lanes by construction (loop counters, broadcast values): their operands
     // then sit in uniform registers. One elected lane issues. (With the walk in one lane's branch, each product took
@@ -252,54 +260,61 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (128u >> 4) << 24;
     constexpr uint32_t idesc_s = idesc | (kBN >> 3) << 17;
     constexpr uint32_t idesc_o = idesc | 1u << 16 | (D >> 3) << 17;  // V: keys are the slow dimension
-    constexpr uint32_t group8 = 8 * Cfg::kRowBytes, hi = desc_hi(group8, D >= 64 ? 2 : 4);
+    constexpr uint32_t group8 = 8 * KV::kRowBytes, hi = desc_hi(group8, D >= 64 ? 2 : 4);
     const int h = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), s_col = tm + h * 128, o_at = tm + o_col + h * D;
-    const uint32_t q_desc = desc_lo(base + h * Cfg::kTile, 16);
-    uint32_t stage = 0, phase = 0;  // of the K tile that the next scores read
-    uint32_t np = 0, nq = 0;
-    bool ok = true;
-    auto scores = [&](uint32_t st) {  // S = Q K^T, K in stage st
-      if (elect_one()) {
-        const uint32_t k = desc_lo(kv_base + st * Cfg::kTile, 16);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4 * Cfg::kSub + kk % 4 * 32) >> 4;
-          mma_ss(s_col, q_desc + off, k + off, hi, idesc_s, kk > 0);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), s_col = tm + h * 2 * kBN, o_at = tm + o_col + h * D;
+    const uint32_t q_desc = desc_lo(base + h * Q::kTile, 16);
+    struct Ring {
+      uint32_t stage = 0, phase = 0;
+      __device__ __forceinline__ void advance() {
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1;
         }
-        tc_commit(s_full + 8 * h);
-        tc_commit(kv_empty + 8 * st);
       }
-      __syncwarp();
-    };
-    auto output = [&](uint32_t st, bool add) {  // O (+)= P V, V in stage st
+    } rk, rv;
+    uint32_t ns = 0, np = 0, nq = 0;  // scores issued, weights used, items
+    bool ok = true;
+    auto scores = [&] {  // the next S = Q K^T
       if (elect_one()) {
-        const uint32_t v = desc_lo(kv_base + st * Cfg::kTile, Cfg::kSub);
+        const uint32_t k = desc_lo(k_base + rk.stage * KV::kTile, 16), to = s_col + (ns & 1) * kBN;
 #pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk)
-          mma_ts(o_at, s_col + kk * 8, v + (kk * 2 * group8 >> 4), hi, idesc_o, add || kk > 0);
-        tc_commit(kv_empty + 8 * st);
+        for (int kk = 0; kk < D / 16; ++kk)
+          mma_ss(to, q_desc + ((kk / 4 * Q::kSub + kk % 4 * 32) >> 4), k + ((kk / 4 * KV::kSub + kk % 4 * 32) >> 4), hi, idesc_s,
+                 kk > 0);
+        tc_commit(s_full + 16 * h + 8 * (ns & 1));
+        tc_commit(k_empty + 8 * rk.stage);
       }
       __syncwarp();
+      ++ns;
+      rk.advance();
     };
-    auto commit = [&](uint32_t bar) {
-      if (elect_one()) tc_commit(bar);
-      __syncwarp();
-    };
-    auto advance = [&] {
-      if (++stage == S) {
-        stage = 0;
-        phase ^= 1;
+    auto output = [&](bool skip, bool add) {  // O (+)= the next P V
+      if (elect_one()) {
+        const uint32_t v = desc_lo(v_base + rv.stage * KV::kTile, KV::kSub), p = s_col + (np & 1) * kBN;
+        if (!skip) {
+#pragma unroll
+          for (int kk = 0; kk < kBN / 16; ++kk)
+            mma_ts(o_at, p + kk * 8, v + (kk * 2 * group8 >> 4), hi, idesc_o, add || kk > 0);
+        }
+        tc_commit(pv_done + 16 * h + 8 * (np & 1));
+        tc_commit(v_empty + 8 * rv.stage);
       }
+      __syncwarp();
+      ++np;
+      rv.advance();
     };
     for (; ok && w.get(a, t); w.next(a)) {
       const int take = __shfl_sync(0xffffffffu, w.take, 0);
       if (__shfl_sync(0xffffffffu, t.ntok * a.group <= h * 128 ? 1 : 0, 0)) {
         // Nothing to do for this half, but the stages wait for its word too.
-        for (int i = 0; ok && i < 2 * take; ++i) {
-          ok = wait(kv_full + 8 * stage, phase, gave_up);
-          if (ok && lane == 0) mbar_arrive(kv_empty + 8 * stage);
-          advance();
+        for (int i = 0; ok && i < take; ++i) {
+          ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up);
+          if (ok && lane == 0) mbar_arrive(k_empty + 8 * rk.stage);
+          ok = ok && wait(v_full + 8 * rv.stage, rv.phase, gave_up);
+          if (ok && lane == 0) mbar_arrive(v_empty + 8 * rv.stage);
+          rk.advance();
+          rv.advance();
         }
         continue;
       }
@@ -308,48 +323,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       masked_tiles(a, t, first_unit(t, a.window, kBN) + w.k, j_diag, j_win);
       j_diag = __shfl_sync(0xffffffffu, j_diag, 0);
       j_win = __shfl_sync(0xffffffffu, j_win, 0);
-      ok = wait(kv_full + 8 * stage, phase, gave_up) && wait(q_full + 8 * h, nq++ & 1, gave_up);
+      ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up) && wait(q_full + 8 * h, nq++ & 1, gave_up);
       if (!ok) break;
       tc_fence_after();
-      scores(stage);
+      scores();
+      if (take > 1) {
+        ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up);
+        if (!ok) break;
+        scores();
+      }
       for (int j = 0; j < take; ++j) {
-        const bool more = j + 1 < take;
-        advance();
-        const uint32_t v_st = stage;
-        ok = wait(kv_full + 8 * stage, phase, gave_up);
-        advance();  // the next K, of this item or the next one
-        if (ok && more) ok = wait(kv_full + 8 * stage, phase, gave_up);
-        if (ok) ok = wait(p_full + 8 * h, np++ & 1, gave_up);
+        const bool more = j + 2 < take;
+        ok = wait(v_full + 8 * rv.stage, rv.phase, gave_up);
+        if (ok && more) ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up);
+        if (ok) ok = wait(p_full + 16 * h + 8 * (np & 1), np >> 1 & 1, gave_up);
         if (!ok) break;
         tc_fence_after();
         int skip = 0;
-        if (j >= j_diag || j <= j_win) skip = __shfl_sync(0xffffffffu, *static_cast<volatile int *>(&sh.skip[h]), 0);
-        if (!skip)
-          output(v_st, j > 0);
-        else
-          commit(kv_empty + 8 * v_st);
-        if (more)
-          scores(stage);
-        else
-          commit(o_full + 8 * h);
+        if (j >= j_diag || j <= j_win) skip = __shfl_sync(0xffffffffu, *static_cast<volatile int *>(&sh.skip[h][np & 1]), 0);
+        output(skip != 0, j > 0);
+        if (more) scores();
       }
     }
     if (!ok) {  // products in flight end before tensor memory is freed
-      commit(smem_u32(&sh.drain[h]));
+      if (elect_one()) tc_commit(smem_u32(&sh.drain[h]));
+      __syncwarp();
       for (int i = 0; i < 1 << 20 && !mbar_try(smem_u32(&sh.drain[h]), 0); ++i) {
       }
     }
-   }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    Walk w(a, blockIdx.x);
-    const int h = warp >> 2, wt = tid & 127;  // half, thread of the warpgroup = row of the half
+  } else if (warp < kLoadWarp) {
+    const int h = warp >> 2, wt = tid & 127, row = h * 128 + wt;  // half, thread of the warpgroup = row of the half
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + h * 128, o_addr = tmem + lanes + o_col + h * D;
+    const uint32_t s_addr = tmem + lanes + h * 2 * kBN, o_addr = tmem + lanes + o_col + h * D;
     const float c = a.scale_log2;
-    uint32_t ns = 0, no = 0, nm = 0, units = 0;  // S tiles, items, masked tiles of this half; units of the CTA
-    auto all_wait = [&](uint32_t bar, uint32_t parity) { return wait(bar, parity, gave_up); };
-    bool ok = true;
+    uint32_t ns = 0, nm = 0, tiles = 0;  // S tiles, masked tiles of this half; tiles of the CTA
+    bool ok = true, q_in = false;
+    // Waits for the products of tile ns - 1. (Two barriers in turn: the scores of tile ns - 1 came behind the products
+    // of ns - 3, so that the phase waited for is the only one that can be open.)
+    auto pv_wait = [&] { return wait(pv_done + 16 * h + 8 * ((ns - 1) & 1), (ns - 1) >> 1 & 1, gave_up); };
     // This half's query rows of an item into shared memory, asynchronously.
     auto load_q = [&](const Tile &item, int head) {
       const int n_rows = item.ntok * a.group;
@@ -357,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < D / 8; ++i) {
         const int r = (i * 128 + wt) / (D / 8), j = wt % (D / 8), qr = h * 128 + r, tk = token_of(a, qr);
         const T *src = static_cast<const T *>(a.q) + (item.tok0 + tk) * a.q_stride + (head * a.group + qr - tk * a.group) * D + j * 8;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + h * Cfg::kTile + Cfg::chunk_at(r, j)),
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + h * Q::kTile + Q::chunk_at(r, j)),
                      "l"(qr < n_rows ? src : static_cast<const T *>(a.q)), "r"(qr < n_rows ? 16 : 0)
                      : "memory");
       }
@@ -365,49 +376,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto q_loaded = [&] {
       asm volatile("cp.async.wait_all;" ::: "memory");
       proxy_fence();
-      warp_arrive(q_full + 8 * h);
+      mbar_arrive(q_full + 8 * h);
     };
-    Tile t_next;
-    bool have = w.get(a, t), q_in = false;
-    for (Walk w_next = w; have; w = w_next, t = t_next) {
-      w_next = w;
-      w_next.next(a);
-      const bool more = w_next.get(a, t_next);
-      have = more;
+    for (; w.get(a, t); w.next(a)) {
       const int rows = t.ntok * a.group;
-      const int row = h * 128 + wt;
-      const bool whole = w.whole(t);
-      if (h == 1 && rows <= 128) {
-        units += w.take;
+      if (rows <= h * 128) {
+        tiles += w.take;
         continue;
       }
-      const int64_t pos = t.pos0 + token_of(a, row);
       float m = -INFINITY, l = 0.f;
       if (ok && !q_in) {
         load_q(t, w.head);
         q_loaded();
       }
-      q_in = more && t_next.ntok * a.group > h * 128;  // the next item's rows are loaded behind this one's last scores
-      const int64_t hi = t.pos0 + t.ntok, lo = key_lo(t, a.window);
-      const int64_t u0 = first_unit(t, a.window, kBN) + w.k, key0 = u0 * kBN;
-      int j_diag, j_win;
-      masked_tiles(a, t, u0, j_diag, j_win);
-      const int64_t row_lo = a.window > 0 && pos - a.window + 1 > key0 ? pos - a.window + 1 - key0 : 0;
-      const int see_lo = static_cast<int>(row_lo < (1 << 30) ? row_lo : 1 << 30), see_hi = static_cast<int>(pos + 1 - key0);
-      for (int j = 0; ok && j < w.take; ++j, ++units) {
-        const bool masked = j >= j_diag || j <= j_win;
-        const int seen_lo = see_lo - j * kBN, seen_hi = see_hi - j * kBN;  // keys of the tile that this row sees, if masked
-        ok = all_wait(s_full + 8 * h, ns++ & 1);
-        if (!ok) break;
+      q_in = false;
+      // Keys are counted from the segment's first one.
+      int j_diag, j_win, see_lo, see_hi, v_lo, v_hi;
+      {
+        const int64_t u0 = first_unit(t, a.window, kBN) + w.k, key0 = u0 * kBN, pos = t.pos0 + token_of(a, row);
+        masked_tiles(a, t, u0, j_diag, j_win);
+        const int64_t row_lo = a.window > 0 && pos - a.window + 1 > key0 ? pos - a.window + 1 - key0 : 0;
+        see_lo = static_cast<int>(row_lo < (1 << 30) ? row_lo : 1 << 30);
+        see_hi = static_cast<int>(pos + 1 - key0);
+        const int64_t lo = key_lo(t, a.window) - key0;
+        v_lo = static_cast<int>(lo < 0 ? 0 : lo);
+        v_hi = static_cast<int>(t.pos0 + t.ntok - key0);
+      }
+      // One key tile; false when a wait gave up.
+      auto tile = [&](int j, auto with_mask) -> bool {
+        constexpr bool kMasked = decltype(with_mask)::value;
+        const uint32_t buf = ns & 1, s_at = s_addr + buf * kBN;
+        if (!wait(s_full + 16 * h + 8 * buf, ns >> 1 & 1, gave_up)) return false;
         tc_fence_after();
-        if (q_in && j == w.take - 1) load_q(t_next, w_next.head);
+        if (j == w.take - 1) {  // the scores are done with Q: the next item's rows may come
+          Walk next = w;
+          next.next(a);
+          Tile item;
+          q_in = next.get(a, item) && item.ntok * a.group > h * 128;
+          if (q_in) load_q(item, next.head);
+        }
         float s[kBN];
-#pragma unroll
-        for (int i = 0; i < kBN; i += 32) tc_ld32(s_addr + i, s + i);
+        tc_ld32(s_at, s);
+        tc_ld32(s_at + 32, s + 32);
         tc_wait_ld<kBN>(reinterpret_cast<uint32_t *>(s));
-        if (masked) {
+        if constexpr (kMasked) {
+          const int lo = see_lo - j * kBN, hi = see_hi - j * kBN;
 #pragma unroll
-          for (int i = 0; i < kBN; ++i) s[i] = i >= seen_lo && i < seen_hi ? s[i] : -INFINITY;
+          for (int i = 0; i < kBN; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -422,7 +437,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = to;
           l *= f;
           if (j > 0) {
-#pragma unroll
+            if (!pv_wait()) return false;  // O is at rest
+            tc_fence_after();
+#pragma unroll 1
             for (int i = 0; i < D; i += 32) {
               float o[32];
               tc_ld32(o_addr + i, o);
@@ -435,38 +452,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float mc = m == -INFINITY ? 0.f : -m * c;
         float2 sum[2] = {splat2(0.f), splat2(0.f)};
+        uint32_t p[kBN / 2];  // in place of the scores
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float *x = s + i * 32;
-          uint32_t p[16];  // in place of the scores
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float2 e = __ffma2_rn(make_float2(x[2 * k], x[2 * k + 1]), splat2(c), splat2(mc));
-            if (k % 8 >= 8 - kPolyOf8)
-              e = exp2_poly(e);
-            else
-              e = make_float2(ex2_approx_ftz(e.x), ex2_approx_ftz(e.y));
-            sum[k & 1] = __fadd2_rn(sum[k & 1], e);
-            p[k] = pack2<T>(e.x, e.y);
-          }
-          tc_st16(s_addr + 16 * i, p);
+        for (int k = 0; k < kBN / 2; ++k) {
+          float2 e = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), splat2(c), splat2(mc));
+          if (k % 8 >= 8 - kPolyOf8)
+            e = exp2_poly(e);
+          else
+            e = make_float2(ex2_approx_ftz(e.x), ex2_approx_ftz(e.y));
+          sum[k & 1] = __fadd2_rn(sum[k & 1], e);
+          p[k] = pack2<T>(e.x, e.y);
         }
+        tc_st32(s_at, p);
         l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
-        int poisoned = 0;
-        if (masked) {
-          const uint32_t nv = 2 * units + 1;
-          ok = all_wait(kv_full + 8 * (nv % S), (nv / S) & 1);
-          if (!ok) break;
-          unsigned char *vs = base_p + 2 * Cfg::kTile + (nv % S) * Cfg::kTile;
-          const int64_t key = key0 + j * kBN + wt;  // this thread's V row
+        if constexpr (kMasked) {
+          const uint32_t nv = tiles + j;
+          if (!wait(v_full + 8 * (nv % S), (nv / S) & 1, gave_up)) return false;
+          unsigned char *vs = base_p + (v_base - base) + (nv % S) * KV::kTile;
+          const int vr = wt >> 1, key = j * kBN + vr;  // two threads a V row
           bool bad = false;
-          if (key >= hi || key < lo) {
-            for (int q = 0; q < D / 8; ++q) *reinterpret_cast<uint4 *>(vs + Cfg::chunk_at(wt, q)) = make_uint4(0u, 0u, 0u, 0u);
-          } else {
-            for (int q = 0; q < D / 8; ++q) {
-              const uint4 x = *reinterpret_cast<const uint4 *>(vs + Cfg::chunk_at(wt, q));
-              bad |= non_finite2<T>(x.x) | non_finite2<T>(x.y) | non_finite2<T>(x.z) | non_finite2<T>(x.w);
-            }
+#pragma unroll
+          for (int q = 0; q < D / 16; ++q) {
+            uint4 *x = reinterpret_cast<uint4 *>(vs + KV::chunk_at(vr, 2 * q + (wt & 1)));
+            if (key >= v_hi || key < v_lo)
+              *x = make_uint4(0u, 0u, 0u, 0u);
+            else
+              bad |= non_finite2<T>(x->x) | non_finite2<T>(x->y) | non_finite2<T>(x->z) | non_finite2<T>(x->w);
           }
           proxy_fence();
           // The half's 128 threads agree. Slots are used in turn: the next one is
@@ -474,12 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           volatile int *poison = sh.poison[h];
           if (bad) poison[nm % 3] = 1;
           if (wt == 0) poison[(nm + 1) % 3] = 0;
-          warp_arrive(v_seen + 8 * h);
-          ok = all_wait(v_seen + 8 * h, nm & 1);
-          if (!ok) break;
-          poisoned = poison[nm++ % 3];
+          mbar_arrive(v_seen + 8 * h);
+          if (!wait(v_seen + 8 * h, nm & 1, gave_up)) return false;
+          const int poisoned = poison[nm++ % 3];
+          if (wt == 0) *static_cast<volatile int *>(&sh.skip[h][buf]) = poisoned;
           if (poisoned) {
+            const int lo = see_lo - j * kBN, hi = see_hi - j * kBN;
             tc_wait_st();
+            if (j > 0 && !pv_wait()) return false;
+            tc_fence_after();
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
               float o[32];
@@ -494,16 +508,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int kb = 0; kb < kBN; kb += 8) {
                 uint32_t pw[4];
                 __syncwarp();
-                tc_ld4(s_addr + kb / 2, pw);
+                tc_ld4(s_at + kb / 2, pw);
                 tc_wait_ld<4>(pw);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                  if (kb + k < seen_lo || kb + k >= seen_hi) continue;
+                  if (kb + k < lo || kb + k >= hi) continue;
                   const float2 p2 = unpack2<T>(pw[k / 2]);
                   const float pk = k & 1 ? p2.y : p2.x;
 #pragma unroll
                   for (int q = 0; q < 4; ++q) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(vs + Cfg::chunk_at(kb + k, i / 8 + q));
+                    const uint4 x = *reinterpret_cast<const uint4 *>(vs + KV::chunk_at(kb + k, i / 8 + q));
                     const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -519,22 +533,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (masked && wt == 0) *static_cast<volatile int *>(&sh.skip[h]) = poisoned;
         tc_wait_st();
         tc_fence_before();
-        warp_arrive(p_full + 8 * h);
-        if (q_in && j == w.take - 1) q_loaded();
+        mbar_arrive(p_full + 16 * h + 8 * buf);
+        ++ns;
+        return true;
+      };
+      // Tiles with a mask stand at either end; those between them run in a loop without that code.
+      for (int j = 0; ok && j < w.take;) {
+        for (; ok && j < w.take && (j <= j_win || j >= j_diag); ++j) ok = tile(j, std::true_type{});
+        for (; ok && j < w.take && j > j_win && j < j_diag; ++j) ok = tile(j, std::false_type{});
       }
-      if (ok) ok = all_wait(o_full + 8 * h, no++ & 1);
+      tiles += w.take;
+      if (ok && q_in) q_loaded();
+      ok = ok && pv_wait();
       if (!ok && wt == 0 && a.err_flag != nullptr) atomicOr(a.err_flag, XN_DEVERR_WAIT);
       tc_fence_after();
+      const bool whole = w.whole(t), none = t.pos0 + token_of(a, row) < 0;
       // Rows out: a thread writes its row. After a wait that gave up: NaN.
       const float nan = __int_as_float(0x7fc00000);
       float *part_o = partial_of(a, blockIdx.x, w.first ? 0 : 1, kBM, D);
       const int tk = token_of(a, row);
       T *dst = static_cast<T *>(a.out) + (static_cast<int64_t>(t.tok0 + tk) * a.h + w.head * a.group + row - tk * a.group) * D;
       const float inv = __fdiv_rn(1.f, l);
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < D; i += 32) {
         float o[32];
         __syncwarp();
@@ -548,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (row >= rows) continue;
         if (whole) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = pos < 0 ? 0.f : o[k] * inv;
+          for (int k = 0; k < 32; ++k) o[k] = none ? 0.f : o[k] * inv;
 #pragma unroll
           for (int k = 0; k < 32; k += 8)
             st_vec(dst + i + k, make_uint4(pack2<T>(o[k], o[k + 1]), pack2<T>(o[k + 2], o[k + 3]), pack2<T>(o[k + 4], o[k + 5]),

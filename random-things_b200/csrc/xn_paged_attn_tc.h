@@ -7,7 +7,7 @@ namespace xn {
 namespace paged {
 
 // Rows of a query tile and keys of a key tile: chunks, and single tokens.
-constexpr int kTcRows = 256, kTcKeys = 128;
+constexpr int kTcRows = 256, kTcKeys = 64;
 constexpr int kDecRows = 16, kDecKeys = 64;
 
 // Enqueue the kernel for chunks / for single tokens (bf16 / f16); XN_OK, or the error recorded.
