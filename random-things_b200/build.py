@@ -1,4 +1,5 @@
-"""Builds libxn_fused.so, the sm_100a fused layer-op library, in-tree.
+"""Builds libxn_fused.so, the sm_100a fused layer-op library, in-tree, and
+xn_torch.so, the part of the Python binding that is a CPython extension.
 
 Usage: python random-things_b200/build.py [--force] [--verbose]
 
@@ -22,6 +23,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO / "include"
 BUILD_DIR = PKG_DIR / "_build"
 LIB_PATH = PKG_DIR / "libxn_fused.so"
+BINDING_PATH = PKG_DIR / "xn_torch.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # -fmad=false: the reference CPU backend never fuses a*b+c, so neither may the
@@ -96,6 +98,31 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     return LIB_PATH
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """host/xn_torch.cpp against this Python's torch, linked with libxn_fused.so
+    next to it."""
+    import sysconfig
+
+    from torch.utils import cpp_extension
+
+    src = PKG_DIR / "host" / "xn_torch.cpp"
+    newest = max(src.stat().st_mtime, (INCLUDE / "xn_fused.h").stat().st_mtime, LIB_PATH.stat().st_mtime)
+    if not force and BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= newest:
+        return BINDING_PATH
+    cxx = host_compiler()[1:] or ["g++"]
+    inc = [f"-I{p}" for p in (INCLUDE, sysconfig.get_paths()["include"], *cpp_extension.include_paths(device_type="cuda"))]
+    lib = [f"-L{p}" for p in cpp_extension.library_paths(device_type="cuda")]
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [*cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=xn_torch", *inc, str(src),
+           "-o", str(tmp), f"-L{PKG_DIR}", "-lxn_fused", "-Wl,-rpath,$ORIGIN", *lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
+
+
 def main(argv: list[str] | None = None) -> int:
     ap = argparse.ArgumentParser(description=__doc__)
     ap.add_argument("--force", action="store_true")
@@ -104,6 +131,7 @@ def main(argv: list[str] | None = None) -> int:
     a = ap.parse_args(argv)
     path = build(force=a.force, verbose=a.verbose, ptxas_verbose=a.ptxas_verbose)
     print(path)
+    print(build_binding(force=a.force, verbose=a.verbose))
     return 0
 
 

@@ -106,6 +106,29 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The compiled part of this binding (host/xn_torch.cpp), next to the
+    library: the checks and calls of the operators whose callers count
+    microseconds. Fails loudly when it has not been built."""
+    global _binding
+    if _binding is None:
+        import importlib.util
+
+        lib()
+        path = LIB_PATH.with_name("xn_torch.so")
+        if not path.exists():
+            raise XnError(f"{path} is not built: run `python random-things_b200/build.py`")
+        spec = importlib.util.spec_from_file_location("xn_torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.set_error(XnError)
+        _binding = mod
+    return _binding
+
+
 def last_error() -> str:
     return lib().xn_last_error().decode()
 
@@ -788,43 +811,6 @@ def position_advance(total_dev: torch.Tensor, t: int) -> None:
 # reference counterpart; the reference's caches hold one position per batch)
 # ---------------------------------------------------------------------------
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    # The launch goes to the tensors' device, which need not be the current one.
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        _call(name, *args)
-    else:
-        with torch.cuda.device(dev):
-            _call(name, *args)
-
-
-def _ints(op: str, dtype: torch.dtype, **ts: torch.Tensor) -> None:
-    for name, t in ts.items():
-        if t.dtype != dtype:
-            raise XnError(f"{op}: {name} must be {dtype}, got {t.dtype}", XN_E_DTYPE)
-
-
-def _err_word(op: str, err_flag: torch.Tensor | None) -> None:
-    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() < 1):
-        raise XnError(f"{op}: err_flag must be an int32 CUDA tensor")
-
-
-def _pool(op: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int, int, int, int]:
-    """(n_pages, h_kv, page_size, d, page stride, head stride, slot stride) of a pool seen as
-    [n_pages, h_kv, page_size, d]; a pool laid out otherwise is passed as a permuted view."""
-    _check_same_shape(k_pages.shape, v_pages.shape, f"{op} pools")
-    if k_pages.dim() != 4:
-        raise XnError(f"{op}: pools must be [n_pages, h_kv, page_size, d], got {tuple(k_pages.shape)}")
-    if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
-        raise XnError(f"{op}: pools must share their strides and have a unit last stride")
-    return (*k_pages.shape, *k_pages.stride()[:3])
-
-
-def _on_device(ref: torch.Tensor, op: str, *ts: torch.Tensor | None) -> None:
-    for t in ts:
-        if t is not None and (not t.is_cuda or t.device != ref.device):
-            raise XnError(f"{op}: tensors must be on one CUDA device")
-
-
 class PagedPlan(NamedTuple):
     """A step's bookkeeping (paged_plan): where each request's tokens begin, the
     lengths after the step, each token's position and slot (-1: padding), and
@@ -849,31 +835,9 @@ def paged_plan(lens: torch.Tensor, new_len: torch.Tensor, block_table: torch.Ten
     fit changes nothing, sets XN_DEVERR_FULL in err_flag and gives an empty
     plan (q_start 0, slots -1); contradictory inputs set XN_DEVERR_RANGE.
     No host synchronisation: a captured graph may hold the call."""
-    op = "paged_plan"
-    if lens.dim() != 1 or block_table.dim() != 2 or free_ring.dim() != 1:
-        raise XnError(f"{op}: expected lens [R], block_table [R, blocks], free_ring [n_pages]")
-    n, blocks = block_table.shape
-    _check_same_shape(lens.shape, (n,), f"{op} lens")
-    _check_same_shape(new_len.shape, (n,), f"{op} new_len")
-    _check_same_shape(ring_state.shape, (2,), f"{op} ring_state")
-    if token_cap < 0:
-        raise XnError(f"{op}: negative token_cap")
-    dev = _dev(lens, new_len, block_table, free_ring, ring_state, err_flag)
-    if out is None:
-        # One buffer for all five: small calls are bound by their launches.
-        buf = torch.empty(2 * n + 1 + 2 * token_cap + 2, dtype=torch.int64, device=dev)
-        out = PagedPlan(*buf.split([n + 1, n, token_cap, token_cap, 2]))
-    for t, shape in zip(out, ((n + 1,), (n,), (token_cap,), (token_cap,), (2,))):
-        _check_same_shape(t.shape, shape, f"{op} out")
-    _dev(lens, *out)
-    _ints(op, torch.int64, lens=lens, new_len=new_len, ring_state=ring_state)
-    _ints(op, torch.int64, **out._asdict())
-    _ints(op, torch.int32, block_table=block_table, free_ring=free_ring)
-    _err_word(op, err_flag)
-    _call_on(dev, "xn_paged_plan", _p(out.q_start), _p(out.kv_len), _p(out.positions), _p(out.slots),
-             _p(out.ring_state), _p(block_table), _p(free_ring), _p(lens), _p(new_len), _p(ring_state), n, blocks,
-             free_ring.numel(), int(page_size), int(token_cap), _p(err_flag), _stream(lens))
-    return out
+    t = (_binding or binding()).paged_plan(lens, new_len, block_table, free_ring, ring_state, page_size, token_cap, out,
+                                           err_flag)
+    return t if out is not None else PagedPlan._make(t)
 
 
 def paged_append_rope(qkv: torch.Tensor, heads: int, kv_heads: int, cos: torch.Tensor, sin: torch.Tensor,
@@ -886,29 +850,8 @@ def paged_append_rope(qkv: torch.Tensor, heads: int, kv_heads: int, cos: torch.T
     slot -1 is padding: its q row and the pools are left as they were. Unlike
     kv_append_rope, which repeats the reference's rounding of every product,
     the rotation is f32 with one rounding."""
-    op = "paged_append_rope"
-    n_pages, hk, page, d, ps, hs, ss = _pool(op, k_pages, v_pages)
-    n = positions.numel()
-    if hk != kv_heads or qkv.numel() != n * (heads + 2 * kv_heads) * d or qkv.shape[0] != n:
-        raise XnError(f"{op}: expected qkv [{n}, ({heads} + 2 * {kv_heads}) * {d}] and {kv_heads} kv heads in the pools, "
-                      f"got {tuple(qkv.shape)} and {hk}")
-    _check_same_shape(slots.shape, positions.shape, f"{op} slots")
-    _check_same_shape(cos.shape, sin.shape, f"{op} cos/sin")
-    if cos.dim() != 2 or cos.shape[1] * 2 != d:
-        raise XnError(f"{op}: cos/sin must be [max_pos, {d // 2}], got {tuple(cos.shape)}")
-    if q_out is None:
-        q_out = torch.empty((n, heads, d), dtype=qkv.dtype, device=qkv.device)
-    else:
-        _check_same_shape(q_out.shape, (n, heads, d), f"{op} q_out")
-    dev = _dev(qkv, cos, sin, positions, slots, q_out, err_flag)
-    _on_device(qkv, op, k_pages, v_pages)
-    _same_dtype(qkv, cos, sin, k_pages, v_pages, q_out)
-    _ints(op, torch.int64, positions=positions, slots=slots)
-    _err_word(op, err_flag)
-    _call_on(dev, "xn_paged_append_rope", _p(q_out), _p(k_pages), _p(v_pages), _p(qkv), _p(cos), _p(sin), _p(positions),
-             _p(slots), n, heads, kv_heads, d, cos.shape[0], n_pages, page, ps, hs, ss, int(interleaved),
-             _dtype_code(qkv), _p(err_flag), _stream(qkv))
-    return q_out
+    return (_binding or binding()).paged_append_rope(qkv, heads, kv_heads, cos, sin, k_pages, v_pages, positions, slots,
+                                                     interleaved, err_flag, q_out)
 
 
 def paged_attention_workspace(n_tokens: int, requests: int, heads: int, kv_heads: int, head_dim: int, max_new: int,
@@ -937,35 +880,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     negative position gives zeros. max_new is the largest number of new tokens
     of a request that the caller expects; it decides the kernel, not the
     result. Pages outside the pool read as zeros and set XN_DEVERR_RANGE."""
-    op = "paged_attention"
-    n_pages, hk, page, d, ps, hs, ss = _pool(op, k_pages, v_pages)
-    if q.dim() != 3 or q.shape[2] != d or hk == 0 or q.shape[1] % hk:
-        raise XnError(f"{op}: q must be [N, H, {d}] with H a multiple of {hk}, got {tuple(q.shape)}")
-    n, h, _ = q.shape
-    if n > 0 and (q.stride(2) != 1 or (h > 1 and q.stride(1) != d)):
-        raise XnError(f"{op}: the rows of q must be contiguous")
-    if block_table.dim() != 2:
-        raise XnError(f"{op}: block_table must be [R, blocks], got {tuple(block_table.shape)}")
-    r, blocks = block_table.shape
-    _check_same_shape(kv_len.shape, (r,), f"{op} kv_len")
-    _check_same_shape(q_start.shape, (r + 1,), f"{op} q_start")
-    if out is None:
-        out = torch.empty((n, h * d), dtype=q.dtype, device=q.device)
-    elif out.numel() != n * h * d:
-        raise XnError(f"{op}: out must hold [N, H * D]")
-    if workspace is None:
-        workspace = paged_attention_workspace(n, r, h, hk, d, max_new, q.dtype, q.device)
-    dev = _dev(out, block_table, q_start, kv_len, workspace, err_flag)
-    _on_device(out, op, q, k_pages, v_pages)
-    _same_dtype(q, k_pages, v_pages, out)
-    _ints(op, torch.int64, q_start=q_start, kv_len=kv_len)
-    _ints(op, torch.int32, block_table=block_table)
-    _err_word(op, err_flag)
-    _call_on(dev, "xn_paged_attention", _p(out), _p(q), _p(k_pages), _p(v_pages), _p(block_table), _p(q_start),
-             _p(kv_len), n, r, h, hk, d, n_pages, page, blocks, q.stride(0) if n > 1 else h * d, ps, hs, ss,
-             int(max_new), int(window), float(scale), _dtype_code(q), _p(workspace),
-             workspace.numel() * workspace.element_size(), _p(err_flag), _stream(out))
-    return out
+    return (_binding or binding()).paged_attention(q, k_pages, v_pages, block_table, q_start, kv_len, scale, max_new, window,
+                                                   workspace, err_flag, out)
 
 
 # ---------------------------------------------------------------------------
@@ -980,33 +896,7 @@ def rms_norm_q8(x: torch.Tensor, alpha: torch.Tensor, eps: float, *, branch: tor
     scales [rows]) or per `group` = 32, 64 or 128 columns (scales
     [rows, cols / group]). h is x itself without a branch; otherwise it is
     written to residual_out (which may be x or branch) or a new tensor."""
-    op = "rms_norm_q8"
-    if eps <= 0.0:
-        raise XnError(f"{op} eps must be positive")
-    rows, cols = _rows_cols(x)
-    if group not in (0, 32, 64, 128) or (group and cols % group):
-        raise XnError(f"{op}: group {group} is not 0, 32, 64 or 128 and a divisor of {cols}")
-    _check_same_shape(alpha.shape, (cols,), f"{op} alpha")
-    if branch is not None:
-        _check_same_shape(branch.shape, x.shape, f"{op} branch")
-        if residual_out is None:
-            residual_out = torch.empty_like(x)
-    if residual_out is not None:
-        _check_same_shape(residual_out.shape, x.shape, f"{op} residual_out")
-    shape = (*x.shape[:-1], cols // group) if group else x.shape[:-1]
-    if out is None:
-        out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    if scales is None:
-        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
-    _check_same_shape(out.shape, x.shape, f"{op} out")
-    _check_same_shape(scales.shape, shape, f"{op} scales")
-    dev = _dev(x, alpha, branch, out, scales, residual_out)
-    _same_dtype(x, alpha, branch, residual_out)
-    if out.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
-        raise XnError(f"{op}: out must be float8_e4m3fn and scales float32", XN_E_DTYPE)
-    _call_on(dev, "xn_rms_norm_q8", _p(out), _p(scales), _p(residual_out), _p(x), _p(alpha), _p(branch), rows, cols,
-             int(group), float(eps), _dtype_code(x), _stream(x))
-    return out, scales, x if residual_out is None else residual_out
+    return (_binding or binding()).rms_norm_q8(x, alpha, eps, branch, group, out, scales, residual_out)
 
 
 # ---------------------------------------------------------------------------
