@@ -10,6 +10,8 @@
 // own type), y's f32 operations, and the one to e4m3.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "xn_common.cuh"
 #include "xn_internal.h"
 
@@ -26,133 +28,202 @@ struct Q8Params {
   float eps;
 };
 
-// |y| as a whole number: the order of magnitudes, with NaN above infinity, so
-// that a NaN is the largest of its group.
-__device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
+// The larger of magnitudes; NaN if one is NaN, so that a NaN reaches its group's scale.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
-__device__ __forceinline__ uint32_t umax2(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// mag / 448, correctly rounded for normal results: one FMA step on the product
+// with the rounded reciprocal (an infinite mag has no remainder).
+__device__ __forceinline__ float scale_of(float mag) {
+  constexpr float r = 1.f / 448.f;
+  const float q = __fmul_rn(mag, r);
+  return isinf(mag) ? mag : __fmaf_rn(__fmaf_rn(-448.f, q, mag), r, q);
+}
 
-// Multiplies by 1 / scale; a scale too small for its reciprocal divides, a
-// scale of 0 has only zeros.
-struct Scaler {
-  float scale, inv;
-  __device__ __forceinline__ explicit Scaler(uint32_t mag) {
-    scale = __fdiv_rn(__uint_as_float(mag), 448.f);
-    inv = __frcp_rn(scale);
-  }
-  __device__ __forceinline__ float operator()(float y) const {
-    if (scale < 0x1p-100f) return scale == 0.f ? 0.f : __fdiv_rn(y, scale);
-    return __fmul_rn(y, inv);
+// What y is multiplied with: 1 / scale; 0 for scale 0, whose y are all 0. A
+// scale below 2^-100 may have no f32 reciprocal: `up` first lifts y by 2^64.
+struct Inverse {
+  float inv;
+  bool up;
+  __device__ __forceinline__ explicit Inverse(float scale) {
+    up = scale < 0x1p-100f;
+    inv = scale == 0.f ? 0.f : __frcp_rn(up ? scale * 0x1p64f : scale);
   }
 };
 
-__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-}
+__device__ __forceinline__ uint32_t e4m3x2(float2 v) { return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3); }
 
-// Largest value over a row group of tpr threads (as group_sum).
-__device__ __forceinline__ uint32_t row_umax(uint32_t v, int tpr, uint32_t *red) {
+// Largest magnitude over a row group of tpr threads (as group_sum).
+__device__ __forceinline__ float row_max(float v, int tpr, float *red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
-    if (o < tpr) v = umax2(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (o < tpr) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (tpr <= 32) return v;
   const int warp = threadIdx.x >> 5, wpr = tpr >> 5, first = (warp / wpr) * wpr;
   if ((threadIdx.x & 31) == 0) red[warp] = v;
   __syncthreads();
-  uint32_t s = red[first];
-  for (int w = 1; w < wpr; ++w) s = umax2(s, red[first + w]);
+  float s = red[first];
+  for (int w = 1; w < wpr; ++w) s = max_nan(s, red[first + w]);
   return s;
 }
 
+__device__ __forceinline__ float rstd_of(float sum, int64_t cols, float eps) {
+  return __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(cols)), eps)));
+}
+
+// One access of a row: V elements as float2 pairs (V = 1: the second one 0).
+template <typename T, int V>
+struct Access {
+  static constexpr int kAW = V * static_cast<int>(sizeof(T)) / 4;  // 32-bit words
+  static constexpr int kP = V > 1 ? V / 2 : 1;
+  using Raw = std::conditional_t<V == 1, T, uint4>;  // of a uint4, the kAW low words are in use
+  __device__ __forceinline__ static Raw zero() {
+    if constexpr (V == 1)
+      return Elem<T>::from_f32(0.f);
+    else
+      return make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ static Raw load(const void *base, int64_t at) {
+    const T *p = static_cast<const T *>(base) + at;
+    if constexpr (V == 1)
+      return *p;
+    else
+      return ld_stream_w<kAW>(p);
+  }
+  __device__ __forceinline__ static Raw load_cached(const void *base, int64_t at) {
+    const T *p = static_cast<const T *>(base) + at;
+    if constexpr (V == 1)
+      return *p;
+    else
+      return ld_cached_w<kAW>(p);
+  }
+  __device__ __forceinline__ static void store(void *base, int64_t at, Raw v) {
+    T *p = static_cast<T *>(base) + at;
+    if constexpr (V == 1)
+      *p = v;
+    else
+      st_w<kAW>(p, v);
+  }
+  __device__ __forceinline__ static Raw add(Raw x, Raw b) {
+    if constexpr (V == 1)
+      return Elem<T>::from_f32(__fadd_rn(Elem<T>::to_f32(x), Elem<T>::to_f32(b)));
+    else
+      return residual_vec<T, kAW>(x, b, nullptr);
+  }
+  __device__ __forceinline__ static void unpack(Raw v, float2 (&h)[kP]) {
+    if constexpr (V == 1) {
+      h[0] = make_float2(Elem<T>::to_f32(v), 0.f);
+    } else {
+      float2 all[Pairs<T>::kP];
+      Pairs<T>::unpack(v, all);
+#pragma unroll
+      for (int j = 0; j < kP; ++j) h[j] = all[j];
+    }
+  }
+};
+
 // The row in registers: N accesses of V elements by each of its tpr threads.
-template <typename T, int V, int N>
-__global__ void __launch_bounds__(1024) rms_norm_q8_kernel(const Q8Params p) {
+template <typename T, int V, int N, int kBlock, bool kGroups>
+__global__ void __launch_bounds__(kBlock, kBlock == 256 ? (V * sizeof(T) == 16 ? 4 : 3) : 1) rms_norm_q8_kernel(const Q8Params p) {
   griddep_wait();
   griddep_release();
-  __shared__ float red_sum[32];
-  __shared__ uint32_t red_max[32];
+  using A = Access<T, V>;
+  constexpr int P = A::kP;
+  __shared__ float red_sum[32], red_max[32];
   const int tpr = p.tpr, g = threadIdx.x / tpr, lr = threadIdx.x - g * tpr;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / tpr) + g;
-  const bool live = row < p.rows;
-  const int64_t base = row * p.cols, nvec = p.cols / V;
-  float h[N][V];
-  float sum = 0.f;
+  const int nacc = row < p.rows ? static_cast<int>(p.cols / V) : 0;  // accesses of this row
+  const int64_t base = row * p.cols;
+  float2 h[N][P];
+  {
+    // All loads first: each would otherwise wait for the store before it.
+    typename A::Raw x[N], br[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t c = lr + static_cast<int64_t>(i) * tpr;
-    const bool in = live && c < nvec;
-    if constexpr (V == 1) {
-      float x = in ? ld_elem<T>(p.src, base + c) : 0.f;
-      if (in && p.branch != nullptr) x = Elem<T>::round(__fadd_rn(x, ld_elem<T>(p.branch, base + c)));
-      if (in && p.residual_out != nullptr) st_elem<T>(p.residual_out, base + c, x);
-      h[i][0] = x;
-    } else {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (in) {
-        x = ld_stream(static_cast<const T *>(p.src) + base + c * V);
-        if (p.branch != nullptr) x = residual_vec<T>(x, ld_stream(static_cast<const T *>(p.branch) + base + c * V), nullptr);
-        if (p.residual_out != nullptr) st_vec(static_cast<T *>(p.residual_out) + base + c * V, x);
-      }
-      unpack<T>(x, h[i]);
+    for (int i = 0; i < N; ++i) {
+      const int c = lr + i * tpr;
+      x[i] = c < nacc ? A::load(p.src, base + c * V) : A::zero();
+      if (p.branch != nullptr) br[i] = c < nacc ? A::load(p.branch, base + c * V) : A::zero();
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum = __fmaf_rn(h[i][j], h[i][j], sum);
-  }
-  sum = group_sum<false>(sum, tpr, red_sum);
-  const float rstd = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(p.cols)), p.eps)));
-  uint32_t mag[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t c = lr + static_cast<int64_t>(i) * tpr;
-    float w[V];
-    if constexpr (V == 1) {
-      w[0] = c < nvec ? ld_elem<T>(p.alpha, c) : 0.f;
-    } else {
-      unpack<T>(c < nvec ? ld_cached(static_cast<const T *>(p.alpha) + c * V) : make_uint4(0u, 0u, 0u, 0u), w);
-    }
-    mag[i] = 0;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      h[i][j] = __fmul_rn(__fmul_rn(h[i][j], rstd), w[j]);
-      if (c < nvec) mag[i] = umax2(mag[i], magnitude(h[i][j]));
+    for (int i = 0; i < N; ++i) {
+      const int c = lr + i * tpr;
+      if (p.branch != nullptr) x[i] = A::add(x[i], br[i]);
+      if (c < nacc && p.residual_out != nullptr) A::store(p.residual_out, base + c * V, x[i]);
+      A::unpack(x[i], h[i]);
     }
   }
-  if (p.group == 0) {
-    uint32_t all = 0;
+  typename A::Raw w[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) all = umax2(all, mag[i]);
-    all = row_umax(all, tpr, red_max);
+  for (int i = 0; i < N; ++i) w[i] = lr + i * tpr < nacc ? A::load_cached(p.alpha, (lr + i * tpr) * V) : A::zero();
+  float2 sq = splat2(0.f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) mag[i] = all;
-    if (live && lr == 0) p.scales[row] = Scaler(all).scale;
-  } else if constexpr (V > 1) {
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < P; ++j) sq = __ffma2_rn(h[i][j], h[i][j], sq);
+  const float sum = group_sum<false>(__fadd_rn(sq.x, sq.y), tpr, red_sum);
+  const float rstd = rstd_of(sum, p.cols, p.eps);
+  float mag[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float2 wf[P];
+    A::unpack(w[i], wf);
+    mag[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      h[i][j] = __fmul2_rn(__fmul2_rn(h[i][j], splat2(rstd)), wf[j]);
+      mag[i] = max_nan(mag[i], fabsf(h[i][j].x), V > 1 ? fabsf(h[i][j].y) : 0.f);
+    }
+    if (lr + i * tpr >= nacc) mag[i] = 0.f;  // 0 * inf, where rstd is infinite
+  }
+  float scale[kGroups ? N : 1];
+  if constexpr (!kGroups) {
+    float all = mag[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) all = max_nan(all, mag[i]);
+    scale[0] = scale_of(row_max(all, tpr, red_max));
+    if (nacc > 0 && lr == 0) p.scales[row] = scale[0];
+  } else {
     const int lanes = p.group / V;  // neighbouring lanes of one group; a group is whole or absent
 #pragma unroll
     for (int i = 0; i < N; ++i) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1)
-        if (o < lanes) mag[i] = umax2(mag[i], __shfl_xor_sync(0xffffffffu, mag[i], o));
-      const int64_t c = lr + static_cast<int64_t>(i) * tpr;
-      if (live && c < nvec && lr % lanes == 0) p.scales[row * (nvec / lanes) + c / lanes] = Scaler(mag[i]).scale;
+        if (o < lanes) mag[i] = max_nan(mag[i], __shfl_xor_sync(0xffffffffu, mag[i], o));
+      scale[i] = scale_of(mag[i]);
+      const int c = lr + i * tpr;
+      if (c < nacc && lr % lanes == 0) p.scales[row * (nacc / lanes) + c / lanes] = scale[i];
     }
   }
+  Inverse s(scale[0]);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int64_t c = lr + static_cast<int64_t>(i) * tpr;
-    if (!live || c >= nvec) continue;
-    const Scaler s(mag[i]);
-    uint8_t *dst = p.dst + base + c * V;
-    if constexpr (V == 1) {
-      *dst = static_cast<uint8_t>(e4m3x2(s(h[i][0]), 0.f));
-    } else {
-      uint32_t word[V / 4];
+    const int c = lr + i * tpr;
+    if (kGroups && i > 0) s = Inverse(scale[kGroups ? i : 0]);
+    if (s.up) {
 #pragma unroll
-      for (int j = 0; j < V; j += 4) word[j / 4] = e4m3x2(s(h[i][j]), s(h[i][j + 1])) | e4m3x2(s(h[i][j + 2]), s(h[i][j + 3])) << 16;
-      if constexpr (V == 8)
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(word[0], word[1]);
-      else
-        *reinterpret_cast<uint32_t *>(dst) = word[0];
+      for (int j = 0; j < P; ++j) h[i][j] = __fmul2_rn(h[i][j], splat2(0x1p64f));
     }
+    uint32_t two[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) two[j] = e4m3x2(__fmul2_rn(h[i][j], splat2(s.inv)));
+    if (c >= nacc) continue;
+    uint8_t *dst = p.dst + base + c * V;
+    if constexpr (V == 8)
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+    else if constexpr (V == 4)
+      *reinterpret_cast<uint32_t *>(dst) = two[0] | two[1] << 16;
+    else if constexpr (V == 2)
+      *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(two[0]);
+    else
+      *dst = static_cast<uint8_t>(two[0]);
   }
 }
 
@@ -164,8 +235,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024) rms_norm_q8_loop_kernel(const Q8Params p) {
   griddep_wait();
   griddep_release();
-  __shared__ float red_sum[32];
-  __shared__ uint32_t red_max[32];
+  __shared__ float red_sum[32], red_max[32];
   const int64_t base = static_cast<int64_t>(blockIdx.x) * p.cols;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = p.group;
@@ -182,7 +252,7 @@ __global__ void __launch_bounds__(1024) rms_norm_q8_loop_kernel(const Q8Params p
     sum = __fmaf_rn(x, x, sum);
   }
   sum = group_sum<false>(sum, 1024, red_sum);
-  const float rstd = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(p.cols)), p.eps)));
+  const float rstd = rstd_of(sum, p.cols, p.eps);
   auto y_at = [&](int64_t c) {
     if (c >= p.cols) return 0.f;
     float x;
@@ -194,69 +264,87 @@ __global__ void __launch_bounds__(1024) rms_norm_q8_loop_kernel(const Q8Params p
     }
     return __fmul_rn(__fmul_rn(x, rstd), ld_elem<T>(p.alpha, c));
   };
-  uint32_t all = 0;
+  float all = 0.f;
   if (group == 0) {
-    for (int64_t k = 0; k < per_thread; ++k) all = umax2(all, magnitude(y_at(column(k))));
-    all = row_umax(all, 1024, red_max);
-    if (threadIdx.x == 0) p.scales[blockIdx.x] = Scaler(all).scale;
+    for (int64_t k = 0; k < per_thread; ++k) all = max_nan(all, fabsf(y_at(column(k))));
+    all = row_max(all, 1024, red_max);
+    if (threadIdx.x == 0) p.scales[blockIdx.x] = scale_of(all);
   }
   const int gi = group == 0 ? 4 : group / 32;  // elements of a thread in one group
   for (int64_t k = 0; k < per_thread; k += gi) {
-    float y[4];
-    uint32_t mag = all;
+    float y[4], mag = all;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       y[j] = j < gi ? y_at(column(k + j)) : 0.f;
-      if (group != 0) mag = umax2(mag, magnitude(y[j]));
+      if (group != 0) mag = max_nan(mag, fabsf(y[j]));
     }
     if (group != 0) {
-      mag = __reduce_max_sync(0xffffffffu, mag);
-      if (lane == 0 && column(k) < p.cols) p.scales[blockIdx.x * (p.cols / group) + column(k) / group] = Scaler(mag).scale;
+      mag = row_max(mag, 32, red_max);
+      if (lane == 0 && column(k) < p.cols) p.scales[blockIdx.x * (p.cols / group) + column(k) / group] = scale_of(mag);
     }
-    const Scaler s(mag);
+    const Inverse s(scale_of(mag));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t c = column(k + j);
-      if (j < gi && c < p.cols) p.dst[base + c] = static_cast<uint8_t>(e4m3x2(s(y[j]), 0.f));
+      if (j < gi && c < p.cols)
+        p.dst[base + c] = static_cast<uint8_t>(e4m3x2(make_float2(__fmul_rn(s.up ? y[j] * 0x1p64f : y[j], s.inv), 0.f)));
     }
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, int N, bool kGroups>
+void launch_q8_n(const Q8Params &p, cudaStream_t st) {
+  const int block = p.tpr < 256 ? 256 : p.tpr;
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.rows, int64_t{block} / p.tpr)));
+  if (block == 256)
+    launch_k(rms_norm_q8_kernel<T, V, N, 256, kGroups>, grid, dim3(block), 0, st, p);
+  else
+    launch_k(rms_norm_q8_kernel<T, V, N, 1024, kGroups>, grid, dim3(block), 0, st, p);
+}
+
+// Threads of a row: as few as hold it with n_max accesses each when there are
+// rows enough to fill the GPU; with few rows more of them, down to one access
+// each, since then the row's own latency is the call's time.
+template <typename T, int V, bool kGroups>
 bool launch_q8_rows(Q8Params p, cudaStream_t st) {
-  const int64_t nvec = p.cols / V;
-  int64_t tpr = pow2_ceil(ceil_div(nvec, int64_t{4}));
-  if (tpr > 1024) {
-    if (V > 1 || nvec > 8 * 1024) return false;
-    tpr = 1024;
-  }
-  if (p.group != 0 && tpr < p.group / V) tpr = p.group / V;
-  const int n = static_cast<int>(ceil_div(nvec, tpr));
-  const int block = tpr < 256 ? 256 : static_cast<int>(tpr);
+  constexpr int kMost = V * sizeof(T) == 16 ? 4 : V == 2 ? 8 : 16;
+  const int64_t nacc = p.cols / V;
+  int64_t tpr = pow2_ceil(ceil_div(nacc, int64_t{kMost}));
+  if (tpr > 1024) return false;
+  while (tpr < 1024 && tpr < nacc && p.rows * tpr < int64_t{sm_count()} * 512) tpr *= 2;
+  if (kGroups && tpr < p.group / V) tpr = p.group / V;
+  const int64_t n = ceil_div(nacc, tpr);
   p.tpr = static_cast<int>(tpr);
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.rows, int64_t{block} / tpr)));
   if (n <= 1)
-    launch_k(rms_norm_q8_kernel<T, V, 1>, grid, dim3(block), 0, st, p);
+    launch_q8_n<T, V, 1, kGroups>(p, st);
   else if (n <= 2)
-    launch_k(rms_norm_q8_kernel<T, V, 2>, grid, dim3(block), 0, st, p);
+    launch_q8_n<T, V, 2, kGroups>(p, st);
   else if (n <= 4)
-    launch_k(rms_norm_q8_kernel<T, V, 4>, grid, dim3(block), 0, st, p);
-  else if constexpr (V == 1)
-    launch_k(rms_norm_q8_kernel<T, V, 8>, grid, dim3(block), 0, st, p);
+    launch_q8_n<T, V, 4, kGroups>(p, st);
+  else if constexpr (kMost >= 8) {
+    if (n <= 8)
+      launch_q8_n<T, V, 8, kGroups>(p, st);
+    else if constexpr (kMost >= 16)
+      launch_q8_n<T, V, 16, kGroups>(p, st);
+  }
   return true;
 }
 
 template <typename T>
-int launch_q8(Q8Params p, cudaStream_t st, const char *op) {
+int launch_q8(const Q8Params &p, cudaStream_t st, const char *op) {
+  // The widest access that every row and pointer is aligned to.
+  auto fits = [&](int v) {
+    const uintptr_t bytes = v * sizeof(T);
+    uintptr_t at = reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.alpha) |
+                   reinterpret_cast<uintptr_t>(p.branch) | reinterpret_cast<uintptr_t>(p.residual_out);
+    return p.cols % v == 0 && at % bytes == 0 && reinterpret_cast<uintptr_t>(p.dst) % v == 0;
+  };
   constexpr int V = Elem<T>::kVec;
-  const bool aligned = p.cols % V == 0 && is_aligned16(p.src) && is_aligned16(p.alpha) && is_aligned16(p.dst) &&
-                       (p.branch == nullptr || is_aligned16(p.branch)) &&
-                       (p.residual_out == nullptr || is_aligned16(p.residual_out));
   bool done = false;
-  if (aligned)
-    done = launch_q8_rows<T, V>(p, st);
+  if (fits(V))
+    done = p.group != 0 ? launch_q8_rows<T, V, true>(p, st) : launch_q8_rows<T, V, false>(p, st);
   else if (p.group == 0)
-    done = launch_q8_rows<T, 1>(p, st);
+    done = fits(2) ? launch_q8_rows<T, 2, false>(p, st) : launch_q8_rows<T, 1, false>(p, st);
   if (!done) launch_k(rms_norm_q8_loop_kernel<T>, dim3(static_cast<unsigned>(p.rows)), dim3(1024), 0, st, p);
   return check_launch(op);
 }
