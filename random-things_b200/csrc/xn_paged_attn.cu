@@ -1,5 +1,5 @@
 // xn_paged_attn.cu - causal attention of a step's new tokens over a paged KV
-// cache, for sm_100a: the schedule, the f32 kernel, the join of split work.
+// cache, for sm_100a: the schedule, the f32 kernel and the call.
 //
 //   o = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m),  s_k = scale (q . k),  m = max_k s_k
 //
@@ -13,27 +13,32 @@ namespace xn {
 namespace paged {
 namespace {
 
-constexpr int kSchedThreads = 1024;
+constexpr int kSchedThreads = 512;
 
+// Sum of v over the threads before this one; `all` over all threads.
 __device__ __forceinline__ int64_t block_scan_excl(int64_t v, int64_t *tot, int64_t &all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t s = v;
+  auto scan = [&](int64_t x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += u;
+    }
+    return x;
+  };
+  const int64_t s = scan(v);
   if (lane == 31) tot[warp] = s;
   __syncthreads();
-  int64_t before = 0;
-  all = 0;
-  for (int w = 0; w < kSchedThreads / 32; ++w) {
-    const int64_t t = tot[w];
-    if (w < warp) before += t;
-    all += t;
-  }
+  const int64_t t = scan(lane < kSchedThreads / 32 ? tot[lane] : 0);  // every warp for itself
+  all = __shfl_sync(0xffffffffu, t, 31);
+  const int64_t before = __shfl_sync(0xffffffffu, t, warp > 0 ? warp - 1 : 0);
   __syncthreads();
-  return before + s - v;
+  return (warp > 0 ? before : 0) + s - v;
+}
+
+// x / y and the remainder, in 32 bits where both fit (a 64-bit division takes several times as long).
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  return ((x | y) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y)) : x / y;
 }
 
 // Builds the work list: one block, since it is a few thousand additions.
@@ -41,6 +46,8 @@ __global__ void __launch_bounds__(kSchedThreads) paged_schedule_kernel(const Arg
   griddep_wait();
   griddep_release();
   extern __shared__ int32_t tile_pre[];  // tiles of the requests before request i
+  constexpr int kNear = 1024;
+  __shared__ int64_t near[kNear];  // cstart of the first tiles
   __shared__ int64_t tot[kSchedThreads / 32];
   const int n = a.requests, tid = threadIdx.x;
   int64_t carry = 0, all;
@@ -93,7 +100,10 @@ __global__ void __launch_bounds__(kSchedThreads) paged_schedule_kernel(const Arg
     }
     t.cstart = carry + block_scan_excl(e < n_tiles ? t.units + a.pair_cost : 0, tot, all);
     carry += all;
-    if (e < n_tiles) a.tiles[e] = t;
+    if (e < n_tiles) {
+      a.tiles[e] = t;
+      if (e < kNear) near[e] = t.cstart;
+    }
   }
   const int64_t w = carry * a.h_kv;
   int64_t ctas = (w + a.min_cost - 1) / a.min_cost;
@@ -102,56 +112,100 @@ __global__ void __launch_bounds__(kSchedThreads) paged_schedule_kernel(const Arg
     a.header->ctas = static_cast<int32_t>(ctas);
     a.starts[ctas] = Start{static_cast<int32_t>(n_tiles), 0, 0, 0};
   }
-  // The thread that holds a tile marks the parts that begin in it. A cut in
-  // what a pair costs beyond its units moves to the pair's begin.
-  for (int64_t e = tid; e < n_tiles; e += kSchedThreads) {
-    const Tile t = a.tiles[e];
-    const int64_t pair = t.units + a.pair_cost, lo = t.cstart * a.h_kv, hi = lo + pair * a.h_kv;
-    for (int64_t c = (lo * ctas + w - 1) / w; c < ctas; ++c) {
-      const int64_t r = c * w / ctas - lo;
-      if (r >= hi - lo) break;
-      const int64_t k = r % pair - a.pair_cost;
-      a.starts[c] = Start{static_cast<int32_t>(e), static_cast<int32_t>(r / pair), static_cast<int32_t>(k > 0 ? k : 0), 0};
+  __syncthreads();
+  // A thread a part: the pair and the unit it begins with. A cut in what a pair
+  // costs beyond its units moves to the pair's begin.
+  for (int64_t c = tid; c < ctas; c += kSchedThreads) {
+    const int64_t at = quotient(c * w, ctas);
+    const int64_t one = quotient(at, a.h_kv);  // the tile with cstart <= at / h_kv
+    int64_t lo = 0, hi = n_tiles;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if ((mid < kNear ? near[mid] : a.tiles[mid].cstart) <= one)
+        lo = mid;
+      else
+        hi = mid;
     }
+    const Tile t = a.tiles[lo];
+    const int64_t pair = t.units + a.pair_cost, r = at - t.cstart * a.h_kv, head = quotient(r, pair);
+    const int64_t begin = at - r + head * pair, k = r - head * pair - a.pair_cost;
+    int64_t first = 0;
+    if (k > 0) {
+      // Part i begins at floor(i w / ctas): the first one behind the pair's extra cost, the last one before its end.
+      first = quotient((begin + a.pair_cost + 1) * ctas + w - 1, w);
+      if (first == c) a.cuts[c] = Cut{static_cast<int32_t>(quotient((begin + pair) * ctas + w - 1, w) - 1), 0};
+    }
+    a.starts[c] = Start{static_cast<int32_t>(lo), static_cast<int32_t>(head), static_cast<int32_t>(k > 0 ? k : 0),
+                        static_cast<int32_t>(first)};
   }
 }
 
 // ---------------------------------------------------------------------------
-// Tiles on the CUDA cores: 16 x 16 threads, each with kRows rows and every
-// 16th key (scores) or a run of columns (output).
+// f32 on the CUDA cores: its tensor-core forms round the operands. 16 x 16
+// threads, each with kRows rows and every 16th key (scores) or a run of columns
+// (output). K and V tiles arrive by cp.async, the next one while this one is
+// worked on; key tiles are as long as two tiles of both leave room for two
+// CTAs an SM.
 // ---------------------------------------------------------------------------
 template <int D, int BM>
 struct SimtCfg {
-  static constexpr int kBN = 64, kRows = BM / 16;
-  static constexpr int kQ = BM * D, kK = kBN * (D + 4), kV = kBN * D, kP = BM * (kBN + 4);
-  static constexpr size_t kSmem = sizeof(float) * (kQ + kK + kV + kP);
+  static constexpr int kBN = D == 128 ? 32 : 64, kRows = BM / 16, kKeys = kBN / 16;
+  static constexpr int kK = kBN * (D + 4), kV = kBN * D, kQ = BM * D, kP = BM * (kBN + 4);
+  static constexpr size_t kSmem = sizeof(float) * (2 * (kK + kV) + kQ + kP);
 };
 
 template <int D, int BM>
-__global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
+__global__ void __launch_bounds__(256, 2) paged_attn_simt_kernel(const Args a) {
   griddep_wait();
   griddep_release();
-  using T = float;
   using Cfg = SimtCfg<D, BM>;
-  constexpr int BN = Cfg::kBN, R = Cfg::kRows, V = Elem<T>::kVec, CP = D / 16;
+  constexpr int BN = Cfg::kBN, R = Cfg::kRows, KN = Cfg::kKeys, CP = D / 16, PS = BN + 4;
   extern __shared__ __align__(16) float simt_smem[];
-  float *Qs = simt_smem, *Ks = Qs + Cfg::kQ, *Vs = Ks + Cfg::kK, *Ps = Vs + Cfg::kV;
+  __shared__ int last_piece;
+  float *Qs = simt_smem + 2 * (Cfg::kK + Cfg::kV), *Ps = Qs + Cfg::kQ;
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int part = blockIdx.x;
-  const int64_t page_mask = (int64_t{1} << a.page_shift) - 1;
+  const int page_mask = (1 << a.page_shift) - 1;
   Tile t;
   for (Walk w(a, part); w.get(a, t); w.next(a)) {
     const int rows = t.ntok * a.group;
-    __syncthreads();  // the last segment's reads of Qs are done
-    for (int i = tid; i < BM * (D / V); i += 256) {
-      const int row = i / (D / V), c = i % (D / V) * V;
-      float x[V] = {};
-      if (row < rows) {
-        const int64_t tok = t.tok0 + token_of(a, row), head = w.head * a.group + row - token_of(a, row) * a.group;
-        unpack<T>(ld_cached(static_cast<const T *>(a.q) + tok * a.q_stride + head * D + c), x);
-      }
+    const int64_t key_hi = t.pos0 + t.ntok;  // keys from here on are seen by no row
+    const int64_t lo = key_lo(t, a.window);
+    const int64_t u0 = first_unit(t, a.window, BN) + w.k;
+    // Starts the copies of key tile u0 + j; what no row sees, and pages outside the pool, become zeros.
+    auto load = [&](int j) {
+      float *ks = simt_smem + (j & 1) * (Cfg::kK + Cfg::kV), *vs = ks + Cfg::kK;
 #pragma unroll
-      for (int j = 0; j < V; ++j) Qs[row * D + c + j] = x[j];
+      for (int i = 0; i < BN * (D / 4) / 256; ++i) {
+        const int row = (i * 256 + tid) / (D / 4), c = tid % (D / 4) * 4;
+        const int64_t key = (u0 + j) * BN + row;
+        int64_t at = 0;
+        int bytes = 0;
+        if (key < key_hi && key >= lo) {
+          const int32_t page = a.table[t.req * a.max_blocks + (key >> a.page_shift)];
+          if (page >= 0 && page < a.n_pages) {
+            at = page * a.page_stride + w.head * a.head_stride + (static_cast<int>(key) & page_mask) * a.slot_stride + c;
+            bytes = 16;
+          } else if (a.err_flag != nullptr) {
+            atomicOr(a.err_flag, XN_DEVERR_RANGE);
+          }
+        }
+        const uint32_t kd = static_cast<uint32_t>(__cvta_generic_to_shared(ks + row * (D + 4) + c));
+        const uint32_t vd = static_cast<uint32_t>(__cvta_generic_to_shared(vs + row * D + c));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(kd), "l"(static_cast<const float *>(a.k) + at), "r"(bytes) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(vd), "l"(static_cast<const float *>(a.v) + at), "r"(bytes) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();  // the last segment's reads are done
+    load(0);
+    for (int i = tid; i < BM * (D / 4); i += 256) {
+      const int row = i / (D / 4), c = i % (D / 4) * 4, tk = token_of(a, row);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < rows)
+        x = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (t.tok0 + tk) * a.q_stride +
+                                              (w.head * a.group + row - tk * a.group) * D + c);
+      *reinterpret_cast<float4 *>(&Qs[row * D + c]) = x;
     }
     float o[R][CP], m[R], l[R];
     int64_t pos[R];
@@ -163,48 +217,31 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
 #pragma unroll
       for (int c = 0; c < CP; ++c) o[r][c] = 0.f;
     }
-    const int64_t key_hi = t.pos0 + t.ntok;  // keys from here on are seen by no row
-    const int64_t lo = key_lo(t, a.window);
-    const int64_t u0 = first_unit(t, a.window, BN) + w.k;
-    for (int64_t u = u0; u < u0 + w.take; ++u) {
-      const int64_t key0 = u * BN;
-      __syncthreads();  // the last tile's reads are done
-      for (int i = tid; i < BN * (D / V); i += 256) {
-        const int row = i / (D / V), c = i % (D / V) * V;
-        const int64_t key = key0 + row;
-        float kx[V] = {}, vx[V] = {};
-        if (key < key_hi && key >= lo) {
-          const int32_t page = a.table[t.req * a.max_blocks + (key >> a.page_shift)];
-          if (page >= 0 && page < a.n_pages) {
-            const int64_t at = page * a.page_stride + w.head * a.head_stride + (key & page_mask) * a.slot_stride + c;
-            unpack<T>(ld_cached(static_cast<const T *>(a.k) + at), kx);
-            unpack<T>(ld_cached(static_cast<const T *>(a.v) + at), vx);
-          } else if (a.err_flag != nullptr) {
-            atomicOr(a.err_flag, XN_DEVERR_RANGE);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          Ks[row * (D + 4) + c + j] = kx[j];
-          Vs[row * D + c + j] = vx[j];
-        }
+    for (int j = 0; j < w.take; ++j) {
+      if (j + 1 < w.take) {
+        load(j + 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
       }
       __syncthreads();
-      float s[R][4] = {};
+      const float *Ks = simt_smem + (j & 1) * (Cfg::kK + Cfg::kV), *Vs = Ks + Cfg::kK;
+      const int64_t key0 = (u0 + j) * BN;
+      float s[R][KN] = {};
 #pragma unroll 4
       for (int d = 0; d < D; d += 4) {
-        float4 kf[4];
+        float4 kf[KN];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kf[j] = *reinterpret_cast<const float4 *>(&Ks[(tx + 16 * j) * (D + 4) + d]);
+        for (int k = 0; k < KN; ++k) kf[k] = *reinterpret_cast<const float4 *>(&Ks[(tx + 16 * k) * (D + 4) + d]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const float4 qf = *reinterpret_cast<const float4 *>(&Qs[(ty * R + r) * D + d]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[r][j] = __fmaf_rn(qf.x, kf[j].x, s[r][j]);
-            s[r][j] = __fmaf_rn(qf.y, kf[j].y, s[r][j]);
-            s[r][j] = __fmaf_rn(qf.z, kf[j].z, s[r][j]);
-            s[r][j] = __fmaf_rn(qf.w, kf[j].w, s[r][j]);
+          for (int k = 0; k < KN; ++k) {
+            s[r][k] = __fmaf_rn(qf.x, kf[k].x, s[r][k]);
+            s[r][k] = __fmaf_rn(qf.y, kf[k].y, s[r][k]);
+            s[r][k] = __fmaf_rn(qf.z, kf[k].z, s[r][k]);
+            s[r][k] = __fmaf_rn(qf.w, kf[k].w, s[r][k]);
           }
         }
       }
@@ -212,27 +249,27 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
       const bool masked = key0 + BN - 1 > t.pos0 || (a.window > 0 && key0 <= key_hi - 1 - a.window);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        bool seen[4];
+        bool seen[KN];
         float mx = m[r];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t key = key0 + tx + 16 * j;
-          seen[j] = !masked || (key <= pos[r] && (a.window == 0 || key > pos[r] - a.window));
-          if (seen[j]) mx = fmaxf(mx, s[r][j]);
+        for (int k = 0; k < KN; ++k) {
+          const int64_t key = key0 + tx + 16 * k;
+          seen[k] = !masked || (key <= pos[r] && (a.window == 0 || key > pos[r] - a.window));
+          if (seen[k]) mx = fmaxf(mx, s[r][k]);
         }
 #pragma unroll
-        for (int b = 8; b > 0; b >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, b));
+        for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
         const float base = mx == -INFINITY ? 0.f : mx;
         const float shrink = ex2_approx((m[r] - base) * a.scale_log2);
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = seen[j] ? ex2_approx((s[r][j] - base) * a.scale_log2) : 0.f;
+        for (int k = 0; k < KN; ++k) {
+          const float p = seen[k] ? ex2_approx((s[r][k] - base) * a.scale_log2) : 0.f;
           sum += p;
-          Ps[(ty * R + r) * (BN + 4) + tx + 16 * j] = seen[j] ? p : -1.f;  // -1: no part in the row
+          Ps[(ty * R + r) * PS + tx + 16 * k] = seen[k] ? p : -1.f;  // -1: no part in the row
         }
 #pragma unroll
-        for (int b = 8; b > 0; b >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, b);
+        for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         m[r] = mx;
         l[r] = __fmaf_rn(l[r], shrink, sum);
 #pragma unroll
@@ -241,17 +278,23 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
       __syncwarp();  // a row's weights are written and read by one half warp
       auto weigh = [&](auto with_mask) {
 #pragma unroll 2
-        for (int k = 0; k < BN; ++k) {
-          float vf[CP];
+        for (int k = 0; k < BN; k += 4) {
+          float4 p[R];
 #pragma unroll
-          for (int c = 0; c < CP; ++c) vf[c] = Vs[k * D + (CP >= 4 ? (c / 4) * 64 + tx * 4 + c % 4 : tx * CP + c)];
+          for (int r = 0; r < R; ++r) p[r] = *reinterpret_cast<const float4 *>(&Ps[(ty * R + r) * PS + k]);
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float p = Ps[(ty * R + r) * (BN + 4) + k];
+          for (int i = 0; i < 4; ++i) {
+            float vf[CP];
 #pragma unroll
-            for (int c = 0; c < CP; ++c) {
-              const float x = __fmaf_rn(p, vf[c], o[r][c]);
-              o[r][c] = decltype(with_mask)::value && p < 0.f ? o[r][c] : x;
+            for (int c = 0; c < CP; ++c) vf[c] = Vs[(k + i) * D + (CP >= 4 ? (c / 4) * 64 + tx * 4 + c % 4 : tx * CP + c)];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              const float pk = i == 0 ? p[r].x : i == 1 ? p[r].y : i == 2 ? p[r].z : p[r].w;
+#pragma unroll
+              for (int c = 0; c < CP; ++c) {
+                const float x = __fmaf_rn(pk, vf[c], o[r][c]);
+                o[r][c] = decltype(with_mask)::value && pk < 0.f ? o[r][c] : x;
+              }
             }
           }
         }
@@ -260,6 +303,7 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
         weigh(std::true_type{});
       else
         weigh(std::false_type{});
+      __syncthreads();  // before the tile after the next one takes this one's place
     }
     const bool whole = w.whole(t);
     float *part_o = whole ? nullptr : partial_of(a, part, w.first ? 0 : 1, BM, D);
@@ -267,14 +311,14 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
     for (int r = 0; r < R; ++r) {
       const int row = ty * R + r;
       if (row >= rows) continue;
-      const float inv = pos[r] < 0 ? 0.f : __fdiv_rn(1.f, l[r]);
-      const int64_t tok = t.tok0 + token_of(a, row), head = w.head * a.group + row - token_of(a, row) * a.group;
-      T *dst = static_cast<T *>(a.out) + (tok * a.h + head) * D;
+      const float inv = __fdiv_rn(1.f, l[r]);
+      const int tk = token_of(a, row);
+      float *dst = static_cast<float *>(a.out) + (static_cast<int64_t>(t.tok0 + tk) * a.h + w.head * a.group + row - tk * a.group) * D;
 #pragma unroll
       for (int c = 0; c < CP; ++c) {
         const int col = CP >= 4 ? (c / 4) * 64 + tx * 4 + c % 4 : tx * CP + c;
         if (whole)
-          dst[col] = Elem<T>::from_f32(pos[r] < 0 ? 0.f : o[r][c] * inv);
+          dst[col] = pos[r] < 0 ? 0.f : o[r][c] * inv;
         else
           part_o[row * D + col] = o[r][c];
       }
@@ -283,56 +327,7 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const Args a) {
         part_o[BM * D + BM + row] = l[r];
       }
     }
-  }
-}
-
-// Adds the partial sums of the (tile, head) pairs that were cut, pieces in key
-// order. Block (c, y): the pair cut first at the start of part c + 1, rows from y on.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const Args a, int bm) {
-  griddep_wait();
-  griddep_release();
-  const int c = blockIdx.x + 1, ctas = a.header->ctas;
-  if (c >= ctas) return;
-  const Start s = a.starts[c], b = a.starts[c - 1];
-  if (s.k == 0) return;  // nothing is cut here
-  const bool same = b.tile == s.tile && b.head == s.head;
-  if (same && b.k > 0) return;  // cut before: an earlier block's
-  int last = c;                 // the last part with a piece of the pair
-  while (last + 1 < ctas) {
-    const Start n = a.starts[last + 1];
-    if (n.tile != s.tile || n.head != s.head || n.k == 0) break;
-    ++last;
-  }
-  const Tile t = a.tiles[s.tile];
-  constexpr int C = D / 4, RB = 128 / C;  // threads of a row, rows of a block
-  const int col = threadIdx.x % C * 4;
-  for (int row = blockIdx.y * RB + threadIdx.x / C; row < t.ntok * a.group; row += gridDim.y * RB) {
-    float mx = -INFINITY;
-    for (int i = c - 1; i <= last; ++i) {
-      const float *p = partial_of(a, i, i == c - 1 && !same ? 1 : 0, bm, D);
-      mx = fmaxf(mx, p[bm * D + row]);
-    }
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-    for (int i = c - 1; i <= last; ++i) {
-      const float *p = partial_of(a, i, i == c - 1 && !same ? 1 : 0, bm, D);
-      const float m = p[bm * D + row];
-      const float f = m == -INFINITY ? 0.f : ex2_approx((m - mx) * a.scale_log2);
-      const float4 x = *reinterpret_cast<const float4 *>(&p[row * D + col]);
-      l = __fmaf_rn(p[bm * D + bm + row], f, l);
-      o.x = __fmaf_rn(x.x, f, o.x);
-      o.y = __fmaf_rn(x.y, f, o.y);
-      o.z = __fmaf_rn(x.z, f, o.z);
-      o.w = __fmaf_rn(x.w, f, o.w);
-    }
-    const int64_t pos = t.pos0 + token_of(a, row);
-    const float inv = __fdiv_rn(1.f, l);
-    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    const int64_t tok = t.tok0 + token_of(a, row), head = s.head * a.group + row - token_of(a, row) * a.group;
-    T *dst = static_cast<T *>(a.out) + (tok * a.h + head) * D + col;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) dst[j] = Elem<T>::from_f32(pos < 0 ? 0.f : y[j]);
+    if (!whole) end_piece<float, D>(a, w, t, part, BM, tid, 256, &last_piece, [] { __syncthreads(); });
   }
 }
 
@@ -341,14 +336,14 @@ struct Shape {
   int bm, bn, parts, pair_cost, min_cost;
 };
 
-Shape shape_of(int64_t group, int64_t max_new, int dtype) {
+Shape shape_of(int64_t group, int64_t max_new, int64_t d, int dtype) {
   const bool few = max_new * group <= 16 && group <= 16;
-  if (dtype == XN_F32) return Shape{few ? 16 : 64, 64, 2 * sm_count(), 1, 4};
+  if (dtype == XN_F32) return Shape{few ? 16 : 64, d == 128 ? 32 : 64, 2 * sm_count(), 1, 3};
   return few ? Shape{kDecRows, kDecKeys, 2 * sm_count(), 2, 6} : Shape{kTcRows, kTcKeys, sm_count(), 6, 10};
 }
 
 struct Layout {
-  int64_t tiles, starts, partial, bytes;
+  int64_t tiles, starts, cuts, partial, bytes;
 };
 
 Layout layout_of(const Shape &s, int64_t n_tokens, int64_t requests, int64_t group, int64_t d) {
@@ -357,7 +352,8 @@ Layout layout_of(const Shape &s, int64_t n_tokens, int64_t requests, int64_t gro
   l.tiles = up(sizeof(Header));
   const int64_t tt = s.bm / group;
   l.starts = l.tiles + up(static_cast<int64_t>(sizeof(Tile)) * (n_tokens / tt + requests));
-  l.partial = l.starts + up(static_cast<int64_t>(sizeof(Start)) * (s.parts + 1));
+  l.cuts = l.starts + up(static_cast<int64_t>(sizeof(Start)) * (s.parts + 1));
+  l.partial = l.cuts + up(static_cast<int64_t>(sizeof(Cut)) * s.parts);
   l.bytes = l.partial + up(static_cast<int64_t>(sizeof(float)) * 2 * s.parts * s.bm * (d + 2));
   return l;
 }
@@ -382,7 +378,6 @@ int launch_attn(const Args &a, const Shape &s, cudaStream_t st, const char *op) 
     constexpr int dtype = std::is_same_v<T, __half> ? XN_F16 : XN_BF16;
     if (const int rc = s.bm == kTcRows ? launch_tc(a, D, dtype, st, op) : launch_dec(a, D, dtype, st, op)) return rc;
   }
-  if (a.parts > 1) launch_k(paged_combine_kernel<T, D>, dim3(a.parts - 1, ceil_div(s.bm, 16)), dim3(128), 0, st, a, s.bm);
   return check_launch(op);
 }
 
@@ -411,7 +406,7 @@ int xn_paged_attention_workspace(int64_t *bytes, int64_t n_tokens, int64_t reque
   const char *op = "xn_paged_attention_workspace";
   if (bytes == nullptr) return fail(XN_E_INVALID, "%s: null output pointer", op);
   if (const int rc = paged::check_sizes(op, n_tokens, requests, h, h_kv, d, max_new, dtype)) return rc;
-  const paged::Shape s = paged::shape_of(h / h_kv, max_new, dtype);
+  const paged::Shape s = paged::shape_of(h / h_kv, max_new, d, dtype);
   *bytes = paged::layout_of(s, n_tokens, requests, h / h_kv, d).bytes;
   return ok();
 }
@@ -441,7 +436,7 @@ int xn_paged_attention(void *out, const void *q, const void *k_pages, const void
   for (const void *ptr : ptrs)
     if (!is_aligned16(ptr)) return fail(XN_E_INVALID, "%s: tensors must be 16-byte aligned", op);
   const int64_t group = h / h_kv;
-  const paged::Shape s = paged::shape_of(group, max_new, dtype);
+  const paged::Shape s = paged::shape_of(group, max_new, d, dtype);
   const paged::Layout l = paged::layout_of(s, n_tokens, requests, group, d);
   if (workspace_bytes < l.bytes)
     return fail(XN_E_INVALID, "%s: workspace of %lld bytes, %lld needed", op, (long long)workspace_bytes, (long long)l.bytes);
@@ -480,6 +475,7 @@ int xn_paged_attention(void *out, const void *q, const void *k_pages, const void
   a.header = reinterpret_cast<paged::Header *>(ws);
   a.tiles = reinterpret_cast<paged::Tile *>(ws + l.tiles);
   a.starts = reinterpret_cast<paged::Start *>(ws + l.starts);
+  a.cuts = reinterpret_cast<paged::Cut *>(ws + l.cuts);
   a.partial = reinterpret_cast<float *>(ws + l.partial);
   cudaStream_t st = as_stream(stream);
   XN_DISPATCH_FLOAT(dtype, {

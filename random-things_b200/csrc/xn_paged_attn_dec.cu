@@ -58,7 +58,7 @@ __device__ __forceinline__ void join_sync() { asm volatile("barrier.cta.sync 1, 
 
 struct Shared {
   uint64_t full[8], empty[8];
-  int gave_up;
+  int gave_up, last_piece;
   float max[kWarps][kBM], sum[kWarps][kBM];
 };
 
@@ -298,9 +298,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       join_sync();  // the buffer, and after the last turn sh.max and sh.sum, are free
     }
-    if (!whole && row < rows && col == 0) {
-      part_o[kBM * D + row] = mx;
-      part_o[kBM * D + kBM + row] = dead ? nan : sum;
+    if (!whole) {
+      if (row < rows && col == 0) {
+        part_o[kBM * D + row] = mx;
+        part_o[kBM * D + kBM + row] = dead ? nan : sum;
+      }
+      end_piece<T, D>(a, w, t, blockIdx.x, kBM, tid, 32 * kWarps, &sh.last_piece, join_sync);
     }
   }
 }

@@ -581,9 +581,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<float4 *>(part_o + row * D + i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
       }
-      if (!whole && row < rows) {
-        part_o[kBM * D + row] = ok ? m : nan;
-        part_o[kBM * D + kBM + row] = ok ? l : nan;
+      if (!whole) {
+        if (row < rows) {
+          part_o[kBM * D + row] = ok ? m : nan;
+          part_o[kBM * D + kBM + row] = ok ? l : nan;
+        }
       }
       tc_fence_before();  // O is read before the next item's products write it
     }
@@ -594,12 +596,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
+// Adds the pieces of the cut pairs: block (c, y) those of the pair that part
+// c + 1 is the first to begin inside, 32 rows. (Done at the end of the last
+// piece instead, as for single tokens, it saved this launch, 16 us, and cost the
+// kernel above 33 to 49 us: its registers are all taken.)
+template <typename T, int D>
+__global__ void __launch_bounds__(128) paged_combine_kernel(const Args a) {
+  griddep_wait();
+  griddep_release();
+  const int c = blockIdx.x + 1;
+  if (c >= a.header->ctas) return;
+  const Start s = a.starts[c];
+  if (s.k == 0 || s.first != c) return;
+  const Tile t = a.tiles[s.tile];
+  const int rows = t.ntok * a.group, row0 = blockIdx.y * 32;
+  if (row0 < rows)
+    combine_rows<T, D>(a, t, s.head, c, a.cuts[c].last, kBM, row0, rows < row0 + 32 ? rows : row0 + 32, threadIdx.x, 128);
+}
+
 template <typename T, int D>
 int launch(const Args &a, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t st, const char *op) {
   constexpr int smem = static_cast<int>(TcCfg<D>::kSmem);
   if (cudaFuncSetAttribute(paged_attn_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch(op);
   launch_k(paged_attn_tc_kernel<T, D>, dim3(a.parts), dim3(kThreads), smem, st, a, kmap, vmap);
+  if (a.parts > 1) launch_k(paged_combine_kernel<T, D>, dim3(a.parts - 1, kBM / 32), dim3(128), 0, st, a);
   return XN_OK;
 }
 
