@@ -424,7 +424,7 @@ XN_API int xn_paged_plan(int64_t *q_start, int64_t *kv_len, int64_t *positions, 
  *   q_out [n_tokens, h, d] = rope(q), pool row slots[k] = rope(k) and v,
  * at positions[k], cos / sin [max_pos, d/2]. Products and sums are f32, with
  * one rounding to T (xn_kv_append_rope rounds each product, as the reference
- * does). A token of slot -1 is padding: nothing of it is read or written. A
+ * does). A token of slot -1 is padding: its q_out row stays as it was. A
  * slot outside the pool or a position outside the tables skips that token and
  * sets XN_DEVERR_RANGE. Two tokens must not share a slot. d is 32, 64 or 128;
  * tensors are 16-byte aligned and strides multiples of 16 bytes.

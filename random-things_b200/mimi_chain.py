@@ -352,3 +352,74 @@ class MimiStreamingDecoder(StreamingDecoderChain):
 
     def _static_input(self, t: int) -> torch.Tensor:
         return torch.zeros((self.batch, self.cfg.n_q, t), dtype=torch.int64, device=self.total_dev.device)
+
+
+class PagedStreamingDecoder:
+    """The decoder transformer for streams of different lengths: streams join,
+    bring any number of new frames per step (their first frames at once, then
+    one at a time), and end, sharing one pool of cache pages per layer. Where
+    StreamingDecoderChain holds one position for its whole batch, here each
+    stream has its own; a frame at position p rotates at p and attends to the
+    last `context` positions (mask "absolute" of StreamingDecoderChain, which a
+    stream of one frame per step matches).
+
+    A step takes its frames packed, stream after stream: x [token_cap, D] and
+    new [streams] (int64 on the device; negative: the stream ends and its pages
+    return). One plan per step serves all layers: paged_plan, then per layer
+    fused LayerNorm, QKV GEMM, paged_append_rope, paged_attention, output GEMM,
+    fused LayerNorm, MLP. Rows behind the last frame are padding: what comes out
+    there means nothing. Nothing waits for the host, so that a captured graph
+    can hold the step; err_flag (int32) tells of steps that did not fit, which
+    change nothing."""
+
+    def __init__(self, cfg: MimiChainConfig, weights: dict[str, torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
+                 streams: int, pages: int, token_cap: int, *, max_new: int | None = None, page_size: int = 16,
+                 max_len: int | None = None, act: str = "gelu_erf", context: int | None = None):
+        if act not in ("gelu_erf", "silu"):
+            raise ValueError(f"unknown activation {act!r}")
+        self.cfg, self.w, self.cos, self.sin, self.act = cfg, weights, cos, sin, act
+        self.context = int(context if context is not None else cfg.context)
+        self.page_size, self.token_cap = page_size, token_cap
+        self.max_new = token_cap if max_new is None else max_new
+        dtype, dev = weights["layers.0.norm1.weight"].dtype, weights["layers.0.norm1.weight"].device
+        H, hd = cfg.num_heads, cfg.head_dim
+        self.scale = 1.0 / math.sqrt(hd)
+        self.k = [torch.zeros((pages, H, page_size, hd), dtype=dtype, device=dev) for _ in range(cfg.num_layers)]
+        self.v = [torch.zeros_like(k) for k in self.k]
+        blocks = -(-(cfg.max_seq_len if max_len is None else max_len) // page_size)
+        self.table = torch.full((streams, blocks), -1, dtype=torch.int32, device=dev)
+        self.ring = torch.arange(pages, dtype=torch.int32, device=dev)
+        self.ring_state = torch.tensor([0, pages], dtype=torch.int64, device=dev)
+        self.lens = torch.zeros(streams, dtype=torch.int64, device=dev)
+        self.err_flag = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.workspace = xn.paged_attention_workspace(token_cap, streams, H, H, hd, self.max_new, dtype, dev)
+
+    def step(self, x: torch.Tensor, new: torch.Tensor) -> torch.Tensor:
+        cfg, w, eps, H = self.cfg, self.w, self.cfg.eps, self.cfg.num_heads
+        plan = xn.paged_plan(self.lens, new, self.table, self.ring, self.ring_state, self.page_size, self.token_cap,
+                             err_flag=self.err_flag)
+        resid = x
+        y = xn.layer_norm(resid, w["layers.0.norm1.weight"], w["layers.0.norm1.bias"], eps)
+        for l in range(cfg.num_layers):
+            p = f"layers.{l}."
+            qkv = torch.matmul(y, w[p + "self_attn.in_proj_weight"].t())
+            q = xn.paged_append_rope(qkv, H, H, self.cos, self.sin, self.k[l], self.v[l], plan.positions, plan.slots,
+                                     interleaved=True, err_flag=self.err_flag)
+            a = xn.paged_attention(q, self.k[l], self.v[l], self.table, plan.q_start, plan.kv_len, self.scale,
+                                   max_new=self.max_new, window=self.context, workspace=self.workspace,
+                                   err_flag=self.err_flag)
+            attn = torch.matmul(a, w[p + "self_attn.out_proj.weight"].t())
+            y2, resid = xn.layer_norm_residual(resid, attn, w[p + "norm2.weight"], w[p + "norm2.bias"], eps,
+                                               layer_scale=w[p + "layer_scale_1.scale"])
+            h = torch.matmul(y2, w[p + "linear1.weight"].t())
+            xn.unary_(h, h, self.act)
+            m = torch.matmul(h, w[p + "linear2.weight"].t())
+            if l + 1 < cfg.num_layers:
+                q_ = f"layers.{l + 1}."
+                y, resid = xn.layer_norm_residual(resid, m, w[q_ + "norm1.weight"], w[q_ + "norm1.bias"], eps,
+                                                  layer_scale=w[p + "layer_scale_2.scale"])
+            else:
+                resid = xn.residual_add(resid, m, w[p + "layer_scale_2.scale"])
+        self.lens.copy_(plan.kv_len)
+        self.ring_state.copy_(plan.ring_state)
+        return resid
