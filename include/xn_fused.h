@@ -426,7 +426,8 @@ XN_API int xn_paged_plan(int64_t *q_start, int64_t *kv_len, int64_t *positions, 
  * one rounding to T (xn_kv_append_rope rounds each product, as the reference
  * does). A token of slot -1 is padding: its q_out row stays as it was. A
  * slot outside the pool or a position outside the tables skips that token and
- * sets XN_DEVERR_RANGE. Two tokens must not share a slot. d is 32, 64 or 128;
+ * sets XN_DEVERR_RANGE. Two tokens must not share a slot, and outputs must not
+ * overlap inputs. d is 32, 64 or 128;
  * tensors are 16-byte aligned and strides multiples of 16 bytes.
  */
 XN_API int xn_paged_append_rope(void *q_out, void *k_pages, void *v_pages, const void *qkv, const void *cos,
