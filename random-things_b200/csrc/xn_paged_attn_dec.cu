@@ -4,7 +4,8 @@
 // Bound by the cache's bytes: each key and value row is read once for all rows
 // of its kv head. A producer warp keeps a ring of 64-key tiles in flight by
 // TMA; two CTAs an SM hold about 190 KB of loads, several times what the
-// memory's latency asks for. Four warps take 16 keys of each tile: scores and
+// memory's latency asks for (64 requests of 500 to 16000 keys, 2.3 GB: 351 us,
+// the measured copy rate). Four warps take 16 keys of each tile: scores and
 // weighted values as 16 x 8 x 16 products on the tensor cores (mma.sync: with
 // 16 rows or fewer the 128-row tcgen05 shape would be mostly padding, and the
 // products are a fraction of the load time), the softmax in registers. Each

@@ -9,8 +9,10 @@
 //   O = O + P V    tcgen05.mma, P in tensor memory (over S), V in shared memory
 // The scores of the next two tiles are issued ahead, so that a half's softmax
 // need not wait for its own products. (With one buffer of 128 keys each half
-// went softmax, products, softmax, ...: 4600 clocks for 256 x 128 against 2048
-// of the products alone.) One more warp loads: K and V tiles come by TMA, a box
+// went softmax, products, softmax, ...: an 8192-token prompt of 32 / 8 heads of
+// 128 took 632 us against 547; now 514, 0.66 of the measured bf16 rate. With
+// keys by 64 the score products read shared memory as fast as it goes, which
+// bounds the kernel together with the exponentials.) One more warp loads: K and V tiles come by TMA, a box
 // per page, swizzled as the MMA reads them, through two rings of stages.
 //
 // O stays in tensor memory for all key tiles. When a row's maximum grows by
