@@ -410,7 +410,7 @@ XN_API int xn_position_advance(int64_t *total_dev, int64_t t, void *stream);
  * they were, kv_len = lens, ring_state_out = ring_state, q_start is all 0 and
  * every position and slot is -1, so that the operators below do nothing.
  * (Page ids are checked where a token's slot needs them: such a token alone
- * gets slot -1.) kv_len and ring_state_out must not be lens and ring_state.
+ * gets slot -1.) The outputs must not overlap lens, new_len and ring_state.
  * requests <= XN_PAGED_MAX_REQUESTS.
  */
 XN_API int xn_paged_plan(int64_t *q_start, int64_t *kv_len, int64_t *positions, int64_t *slots,
@@ -427,8 +427,8 @@ XN_API int xn_paged_plan(int64_t *q_start, int64_t *kv_len, int64_t *positions, 
  * does). A token of slot -1 is padding: its q_out row stays as it was. A
  * slot outside the pool or a position outside the tables skips that token and
  * sets XN_DEVERR_RANGE. Two tokens must not share a slot, and outputs must not
- * overlap inputs. d is 32, 64 or 128;
- * tensors are 16-byte aligned and strides multiples of 16 bytes.
+ * overlap inputs. d is 32, 64 or 128; tensors are 16-byte aligned and strides
+ * multiples of 16 bytes.
  */
 XN_API int xn_paged_append_rope(void *q_out, void *k_pages, void *v_pages, const void *qkv, const void *cos,
                                 const void *sin, const int64_t *positions, const int64_t *slots, int64_t n_tokens,

@@ -314,8 +314,12 @@ int xn_paged_plan(int64_t *q_start, int64_t *kv_len, int64_t *positions, int64_t
       (requests > 0 && max_blocks > 0 && block_table == nullptr) ||
       (token_cap > 0 && (positions == nullptr || slots == nullptr)))
     return fail(XN_E_INVALID, "%s: null pointer", op);
-  if ((requests > 0 && (kv_len == lens || kv_len == new_len)) || ring_state_out == ring_state)
-    return fail(XN_E_INVALID, "%s: kv_len / ring_state_out must not be an input array", op);
+  // Every block reads all lengths and the ring state while others write.
+  const int64_t *in[] = {requests > 0 ? lens : nullptr, requests > 0 ? new_len : nullptr, ring_state};
+  const int64_t *out[] = {q_start, kv_len, positions, slots, ring_state_out};
+  for (const int64_t *i : in)
+    for (const int64_t *o : out)
+      if (i != nullptr && i == o) return fail(XN_E_INVALID, "%s: an output must not be an input array", op);
   int shift = 0;
   while ((int64_t{1} << shift) < page_size) ++shift;
   PlanParams p{q_start, kv_len, positions, slots, ring_state_out, block_table, free_ring, lens, new_len, ring_state,

@@ -27,6 +27,7 @@ def _plan_args(**kw):
     (dict(requests=-1), "negative"), (dict(requests=8193), "exceed"), (dict(page_size=24), "page size"),
     (dict(page_size=4), "page size"), (dict(page_size=512), "page size"), (dict(n_pages=0), "out of range"),
     (dict(token_cap=-1), "negative"), (dict(kv_len=2 * P), "input array"), (dict(ring_out=2 * P), "input array"),
+    (dict(q_start=3 * P), "input array"), (dict(slots=2 * P), "input array"), (dict(positions=3 * P), "input array"),
     (dict(table=None), "null"), (dict(slots=None), "null"), (dict(ring=None), "null"), (dict(max_blocks=1 << 32), "out of range")])
 def test_plan_refusals(xn, kw, text):
     assert _rc(xn, "xn_paged_plan", *_plan_args(**kw)) == xn.XN_E_INVALID
