@@ -19,6 +19,7 @@ namespace {
 // out in other arrays than they came in.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 512;
+constexpr size_t kPlanStaticSmem = 512;  // at least what the kernel declares besides its prefix sums
 
 struct PlanParams {
   int64_t *q_start, *kv_len, *positions, *slots, *ring_out;
@@ -58,6 +59,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
   extern __shared__ int32_t plan_smem[];
   __shared__ int64_t warp_tot[3][kPlanThreads / 32];
   __shared__ int bad_any;
+  static_assert(sizeof(warp_tot) + sizeof(bad_any) + 16 <= kPlanStaticSmem);
   const int n = static_cast<int>(p.requests);
   int32_t *tok_pre = plan_smem, *need_pre = tok_pre + n + 1, *back_pre = need_pre + n + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -325,7 +327,8 @@ int xn_paged_plan(int64_t *q_start, int64_t *kv_len, int64_t *positions, int64_t
   PlanParams p{q_start, kv_len, positions, slots, ring_state_out, block_table, free_ring, lens, new_len, ring_state,
                requests, max_blocks, n_pages, token_cap, shift, err_flag};
   const size_t smem = 3 * static_cast<size_t>(requests + 1) * sizeof(int32_t);
-  if (smem > 48 * 1024 &&
+  // The 48 KB that a block has without asking cover both kinds of shared memory.
+  if (smem + kPlanStaticSmem > 48 * 1024 &&
       cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(3 * (XN_PAGED_MAX_REQUESTS + 1) * sizeof(int32_t))) != cudaSuccess)
     return check_launch(op);

@@ -1,0 +1,57 @@
+"""The paged-cache operators and the 8-bit RMSNorm at the ends of what they
+accept: request counts around a shared-memory limit, scores and scales at the
+ends of f32's range, wide query groups, empty rows."""
+import json
+import os
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+import paged_ref
+from test_paged_gpu import DT, Batch, _plan_state, _run_plan, i64
+
+pytestmark = pytest.mark.gpu
+
+REPO = Path(__file__).resolve().parents[1]
+
+
+def _child(code, *args, **env):
+    """Runs code in a process of its own (nothing launched before it); what it prints last, as JSON."""
+    out = subprocess.run([sys.executable, "-c", code, str(REPO), *map(str, args)], env=dict(os.environ, **env),
+                         capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr[-2000:]
+    return json.loads(out.stdout.strip().splitlines()[-1])
+
+
+# -- plan ------------------------------------------------------------------------
+
+PLAN_CHILD = r"""
+import json, sys
+sys.path[:0] = [sys.argv[1] + "/random-things_b200"]
+import torch
+import xn_fused as xn
+n, dev = int(sys.argv[2]), "cuda:0"
+new = torch.ones(n, dtype=torch.int64, device=dev)
+table = torch.full((n, 1), -1, dtype=torch.int32, device=dev)
+ring = torch.arange(n, dtype=torch.int32, device=dev)
+p = xn.paged_plan(torch.zeros_like(new), new, table, ring, torch.tensor([0, n], device=dev), 8, n)
+ids = torch.arange(n, device=dev)
+print(json.dumps([torch.equal(p.slots, ids * 8), torch.equal(table[:, 0].long(), ids), torch.equal(p.q_start[1:], ids + 1)]))
+"""
+
+
+@pytest.mark.parametrize("n", [4061, 4062, 4095, 4096])
+def test_plan_request_counts_at_the_default_shared_memory(n):
+    """12 bytes a request meet the 48 KB that a block has without asking, of which a few hundred bytes are taken."""
+    assert _child(PLAN_CHILD, n) == [True] * 3
+
+
+def test_plan_request_counts_after_one_another(xn, cuda):
+    for n in (4062, 8192, 4095, 4096, 4061):
+        lens, table, ring, state = _plan_state(n, n, 8, 30, 6, n + 3)
+        new = [i % 3 for i in range(n)]
+        want = paged_ref.plan(lens, new, table, ring, state, 8, sum(new))
+        assert list(want) == list(_run_plan(xn, cuda, lens, new, table, ring, state, 8, sum(new)))
