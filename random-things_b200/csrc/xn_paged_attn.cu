@@ -461,7 +461,8 @@ int xn_paged_attention(void *out, const void *q, const void *k_pages, const void
   a.page_stride = page_stride;
   a.head_stride = head_stride;
   a.slot_stride = slot_stride;
-  a.window = window;
+  // Positions are below 2^31 (max_blocks above): a window as long as that hides nothing, and p - window cannot wrap.
+  a.window = window < int64_t{1} << 31 ? window : 0;
   a.requests = static_cast<int32_t>(requests);
   a.h = static_cast<int32_t>(h);
   a.h_kv = static_cast<int32_t>(h_kv);

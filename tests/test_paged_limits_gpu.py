@@ -55,3 +55,16 @@ def test_plan_request_counts_after_one_another(xn, cuda):
         new = [i % 3 for i in range(n)]
         want = paged_ref.plan(lens, new, table, ring, state, 8, sum(new))
         assert list(want) == list(_run_plan(xn, cuda, lens, new, table, ring, state, 8, sum(new)))
+
+
+# -- attention: windows ----------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("new", [[5, 4, 3], [70, 40, 30]])
+@pytest.mark.parametrize("window", [(1 << 31) - 1, 1 << 31, (1 << 63) - 1])
+def test_attention_windows_longer_than_any_request(xn, cuda, dtype, new, window):
+    """The longest windows hide nothing, tokens at negative positions (kv_len below the new tokens) among them."""
+    b = Batch(cuda, dtype, 4, 2, 64, 16, [0, 0, 50], new, kv=[3, 0, 50 + new[2]])
+    want = b.run(xn)
+    assert torch.equal(b.run(xn, window=window), want)
+    b.check(xn, window=window)
