@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     back_pre[i] += static_cast<int32_t>(before[2]);
   }
   const int64_t head = p.ring_state[0], count = p.ring_state[1];
-  if (head < 0 || head >= p.n_pages || count < 0 || count + carry[2] > p.n_pages) bad |= XN_DEVERR_RANGE;
+  if (head < 0 || head >= p.n_pages || count < 0 || count > p.n_pages - carry[2]) bad |= XN_DEVERR_RANGE;
   if (carry[0] > p.token_cap || carry[1] > count) bad |= XN_DEVERR_FULL;
   if (bad) atomicOr(&bad_any, bad);
   __syncthreads();

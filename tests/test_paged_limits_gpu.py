@@ -57,6 +57,19 @@ def test_plan_request_counts_after_one_another(xn, cuda):
         assert list(want) == list(_run_plan(xn, cuda, lens, new, table, ring, state, 8, sum(new)))
 
 
+@pytest.mark.parametrize("state,lens", [([0, (1 << 63) - 1], [5, 16]), ([0, (1 << 63) - 3], [5, 16]), ([(1 << 63) - 1, 2], [5, 16]),
+                                        ([-(1 << 63), 2], [5, 16]), ([0, -(1 << 63)], [5, 16]), ([0, 2], [(1 << 63) - 1, 16]),
+                                        ([0, 2], [-(1 << 63), 16])])
+@pytest.mark.parametrize("new", [[-1, -1], [-1, 1], [3, -(1 << 63)]])
+def test_plan_state_at_the_ends_of_64_bits(xn, cuda, state, lens, new):
+    """A ring or lengths that cannot be, however large, change nothing."""
+    table, ring = [[0, -1, -1], [1, 2, -1]], [9, 8, 7, 6, 5, 4, 3]
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    got = _run_plan(xn, cuda, lens, new, table, ring, state, 8, 6, err)
+    assert int(err) & xn.XN_DEVERR_RANGE
+    assert list(got) == [[0] * 3, lens, [-1] * 6, [-1] * 6, table, ring, state]
+
+
 # -- attention: windows ----------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DT)
