@@ -317,11 +317,18 @@ int xn_paged_plan(int64_t *q_start, int64_t *kv_len, int64_t *positions, int64_t
       (token_cap > 0 && (positions == nullptr || slots == nullptr)))
     return fail(XN_E_INVALID, "%s: null pointer", op);
   // Every block reads all lengths and the ring state while others write.
-  const int64_t *in[] = {requests > 0 ? lens : nullptr, requests > 0 ? new_len : nullptr, ring_state};
-  const int64_t *out[] = {q_start, kv_len, positions, slots, ring_state_out};
-  for (const int64_t *i : in)
-    for (const int64_t *o : out)
-      if (i != nullptr && i == o) return fail(XN_E_INVALID, "%s: an output must not be an input array", op);
+  struct Range {
+    const int64_t *at;
+    int64_t n;
+  };
+  const Range in[] = {{lens, requests}, {new_len, requests}, {ring_state, 2}};
+  const Range out[] = {{q_start, requests + 1}, {kv_len, requests}, {positions, token_cap}, {slots, token_cap}, {ring_state_out, 2}};
+  auto from = [](const Range &r) { return reinterpret_cast<uintptr_t>(r.at); };
+  auto to = [](const Range &r) { return reinterpret_cast<uintptr_t>(r.at) + static_cast<uintptr_t>(r.n) * sizeof(int64_t); };
+  for (const Range &i : in)
+    for (const Range &o : out)
+      if (i.n > 0 && o.n > 0 && from(i) < to(o) && from(o) < to(i))
+        return fail(XN_E_INVALID, "%s: an output must not overlap an input array", op);
   int shift = 0;
   while ((int64_t{1} << shift) < page_size) ++shift;
   PlanParams p{q_start, kv_len, positions, slots, ring_state_out, block_table, free_ring, lens, new_len, ring_state,

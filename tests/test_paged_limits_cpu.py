@@ -1,0 +1,18 @@
+"""Refusals of the paged-cache operators at the ends of what they accept (none
+of these calls reaches a launch)."""
+import pytest
+
+from test_paged_cpu import _plan_args, _rc
+
+# Arrays of 16 requests at addresses of their own, 4096 bytes apart.
+APART = dict(requests=16, token_cap=32, q_start=4096, kv_len=2 * 4096, positions=3 * 4096, slots=4 * 4096, ring_out=5 * 4096,
+             table=6 * 4096, ring=7 * 4096, lens=8 * 4096, new=9 * 4096, ring_state=10 * 4096)
+
+
+@pytest.mark.parametrize("kw", [dict(kv_len=8 * 4096 + 8), dict(kv_len=8 * 4096 - 8), dict(kv_len=8 * 4096 + 15 * 8),
+                                dict(q_start=9 * 4096 - 16 * 8), dict(positions=8 * 4096 + 8), dict(slots=9 * 4096 - 31 * 8),
+                                dict(ring_out=10 * 4096 - 8), dict(ring_out=8 * 4096 + 15 * 8), dict(slots=10 * 4096 + 8)])
+def test_plan_refuses_outputs_that_begin_or_end_inside_an_input(xn, kw):
+    """One output shifted against an input by a few entries: other blocks would read what one has written."""
+    assert _rc(xn, "xn_paged_plan", *_plan_args(**dict(APART, **kw))) == xn.XN_E_INVALID
+    assert "input array" in xn.last_error()

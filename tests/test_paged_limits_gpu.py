@@ -70,6 +70,23 @@ def test_plan_state_at_the_ends_of_64_bits(xn, cuda, state, lens, new):
     assert list(got) == [[0] * 3, lens, [-1] * 6, [-1] * 6, table, ring, state]
 
 
+def test_plan_outputs_next_to_inputs(xn, cuda):
+    """Arrays of one buffer, one behind the other, do not overlap; shifted by an entry they do."""
+    n, cap = 40, 64
+    lens, table, ring, state = _plan_state(1, n, 8, 30, 6, n + 3)
+    new = [i % 3 for i in range(n)]
+    want = paged_ref.plan(lens, new, table, ring, state, 8, cap)
+    sizes = [n, n, n, n + 1, cap, 2, 2, cap]  # kv_len, lens, new, q_start, positions, ring state out, in, slots
+    kv, le, ne, qs, po, ro, ri, sl = torch.full((sum(sizes),), 5, dtype=torch.int64, device=cuda).split(sizes)
+    le.copy_(i64(lens)), ne.copy_(i64(new)), ri.copy_(i64(state))
+    t, r = torch.tensor(table, dtype=torch.int32, device=cuda), torch.tensor(ring, dtype=torch.int32, device=cuda)
+    p = xn.paged_plan(le, ne, t, r, ri, 8, cap, out=xn.PagedPlan(qs, kv, po, sl, ro))
+    assert list(want) == [x.tolist() for x in (p.q_start, p.kv_len, p.positions, p.slots, t, r, p.ring_state)]
+    both = torch.zeros(n + 1, dtype=torch.int64, device=cuda)
+    with pytest.raises(xn.XnError, match="input array"):
+        xn.paged_plan(both[1:], ne, t, r, ri, 8, cap, out=xn.PagedPlan(qs, both[:-1], po, sl, ro))
+
+
 # -- attention: windows ----------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DT)
