@@ -458,6 +458,12 @@ XN_API int xn_paged_append_rope(void *q_out, void *k_pages, void *v_pages, const
  * least xn_paged_attention_workspace() bytes of these sizes; nothing in it
  * needs to be set, nothing is kept in it between calls, and calls that may run
  * at the same time (other streams, other graphs) need their own.
+ *
+ * The 16-bit kernels wait for their own copies and products, with a limit that
+ * valid arguments cannot reach; rows that a wait left unfinished are NaN (0
+ * where a token sees no key), and XN_DEVERR_WAIT is set. The environment
+ * variable XN_PAGED_WAIT_CLOCKS (read once per process) lowers the limit, for
+ * testing that path.
  */
 XN_API int xn_paged_attention(void *out, const void *q, const void *k_pages, const void *v_pages,
                               const int32_t *block_table, const int64_t *q_start, const int64_t *kv_len,

@@ -7,6 +7,8 @@
 // the sums so far shrink by exp(m_old - m_new), and the tile's terms are added.
 #include <math.h>
 
+#include <cstdlib>
+
 #include "xn_paged_attn_tc.h"
 
 namespace xn {
@@ -361,6 +363,19 @@ Layout layout_of(const Shape &s, int64_t n_tokens, int64_t requests, int64_t gro
   return l;
 }
 
+// Clocks after which a wait of the TMA kernels gives up: kWaitClocks, or the
+// value of the environment variable XN_PAGED_WAIT_CLOCKS (read once per
+// process), a diagnostic that lets a test make the waits give up on valid inputs.
+long long wait_clocks() {
+  static const long long clocks = [] {
+    const char *v = std::getenv("XN_PAGED_WAIT_CLOCKS");
+    if (v == nullptr || *v == '\0') return kWaitClocks;
+    const long long n = std::strtoll(v, nullptr, 10);
+    return n < 0 ? 0 : n < kWaitClocks ? n : kWaitClocks;
+  }();
+  return clocks;
+}
+
 template <int D, int BM>
 void launch_simt(const Args &a, cudaStream_t st) {
   constexpr size_t smem = SimtCfg<D, BM>::kSmem;
@@ -475,6 +490,7 @@ int xn_paged_attention(void *out, const void *q, const void *k_pages, const void
   a.pair_cost = s.pair_cost;
   a.min_cost = s.min_cost;
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  a.wait_clocks = paged::wait_clocks();
   a.err_flag = err_flag;
   a.header = reinterpret_cast<paged::Header *>(ws);
   a.tiles = reinterpret_cast<paged::Tile *>(ws + l.tiles);

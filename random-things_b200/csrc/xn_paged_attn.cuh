@@ -55,6 +55,7 @@ struct Args {
   int32_t requests, h, h_kv, group, group_mul, page_shift;
   int32_t tile_tokens, bn, parts, pair_cost, min_cost;
   float scale_log2;  // scale * log2(e): scores enter exp2
+  long long wait_clocks;  // a wait on a barrier gives up after these; 0: the warps of the softmax do before their first one
   int *err_flag;
   Header *header;
   Tile *tiles;

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       int page = ld.page(a, t, u0 * kBN, lo, hi);
       for (int64_t u = u0; u < u0 + w.take; ++u, ++n) {
         const uint32_t st = n % S, round = n / S;
-        ok = round == 0 || wait(empty + 8 * st, (round - 1) & 1, gave_up);
+        ok = round == 0 || wait(empty + 8 * st, (round - 1) & 1, gave_up, a.wait_clocks);
         if (!ok) break;
         if (lane == 0) mbar_expect(full + 8 * st, 2 * Cfg::kTile);
         __syncwarp();
@@ -111,8 +111,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (u + 1 < u0 + w.take) page = ld.page(a, t, (u + 1) * kBN, lo, hi);
       }
     }
-    if (!ok)  // copies in flight end before the block does
-      for (uint32_t i = n > S ? n - S : 0; i < n; ++i) wait(full + 8 * (i % S), (i / S) & 1, gave_up);
+    // Copies in flight end before the block does.
+    for (uint32_t i = n > S ? n - S : 0; i < n; ++i) drain(full + 8 * (i % S), (i / S) & 1);
     return;
   }
   const int g = lane >> 2, t4 = lane & 3;
@@ -120,7 +120,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   // This lane's row of an 8 x 8 matrix in the loads of K (not transposed) and V (transposed).
   const int k_row = warp * 16 + (lane & 7) + (lane >> 4) * 8, k_chunk = lane >> 3 & 1;
   const int v_row = warp * 16 + (lane & 15), v_chunk = lane >> 4;
-  bool ok = true;
+  bool ok = a.wait_clocks > 0;
+  if (!ok) *gave_up = 1;
   for (; w.get(a, t); w.next(a)) {
     const int rows = t.ntok * a.group;
     uint32_t q[D / 16][4];
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int64_t u0 = first_unit(t, a.window, kBN) + w.k;
     for (int64_t u = u0; u < u0 + w.take; ++u, ++n) {
       const uint32_t st = n % S;
-      ok = ok && wait(full + 8 * st, (n / S) & 1, gave_up);
+      ok = ok && wait(full + 8 * st, (n / S) & 1, gave_up, a.wait_clocks);
       if (!ok) continue;
       const uint32_t ks = base + st * 2 * Cfg::kTile, vs = ks + Cfg::kTile;
       float s[2][4] = {};

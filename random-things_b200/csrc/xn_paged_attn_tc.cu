@@ -27,7 +27,8 @@
 // and others do not holds a non-finite value, the half adds the tile's product
 // on the CUDA cores, each token over its own keys (poisoned tile).
 //
-// Every wait has a time limit; see wait().
+// Every wait has a time limit; see wait(). When one gives up, the rows that are
+// left become NaN, and each role still waits for what it has in flight.
 #include "xn_paged_tma.cuh"
 
 namespace xn {
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     auto load = [&](const CUtensorMap *map, uint32_t ring, uint32_t full, uint32_t empty, uint32_t &n, int64_t key0, int page) {
       const uint32_t st = n % S, round = n / S;
-      ok = ok && (round == 0 || wait(empty + 8 * st, (round - 1) & 1, gave_up));
+      ok = ok && (round == 0 || wait(empty + 8 * st, (round - 1) & 1, gave_up, a.wait_clocks));
       if (!ok) return;
       if (lane == 0) mbar_expect(full + 8 * st, KV::kTile);
       __syncwarp();
@@ -250,10 +251,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       load(&vmap, v_base, v_full, v_empty, nv, (u0 + w.take - 1) * kBN, v_page);
     }
-    if (!ok) {  // copies in flight end before the block does
-      for (uint32_t i = nk > S ? nk - S : 0; i < nk; ++i) wait(k_full + 8 * (i % S), (i / S) & 1, gave_up);
-      for (uint32_t i = nv > S ? nv - S : 0; i < nv; ++i) wait(v_full + 8 * (i % S), (i / S) & 1, gave_up);
-    }
+    // Copies in flight end before the block does.
+    for (uint32_t i = nk > S ? nk - S : 0; i < nk; ++i) drain(k_full + 8 * (i % S), (i / S) & 1);
+    for (uint32_t i = nv > S ? nv - S : 0; i < nv; ++i) drain(v_full + 8 * (i % S), (i / S) & 1);
   } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     // A warp for each half, so that what one waits for does not hold up the other. The whole warp walks along, and
     // what the products need is equal in all lanes by construction (loop counters, broadcast values): their operands
@@ -312,9 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (__shfl_sync(0xffffffffu, t.ntok * a.group <= h * 128 ? 1 : 0, 0)) {
         // Nothing to do for this half, but the stages wait for its word too.
         for (int i = 0; ok && i < take; ++i) {
-          ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up);
+          ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up, a.wait_clocks);
           if (ok && lane == 0) mbar_arrive(k_empty + 8 * rk.stage);
-          ok = ok && wait(v_full + 8 * rv.stage, rv.phase, gave_up);
+          ok = ok && wait(v_full + 8 * rv.stage, rv.phase, gave_up, a.wait_clocks);
           if (ok && lane == 0) mbar_arrive(v_empty + 8 * rv.stage);
           rk.advance();
           rv.advance();
@@ -326,20 +326,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       masked_tiles(a, t, first_unit(t, a.window, kBN) + w.k, j_diag, j_win);
       j_diag = __shfl_sync(0xffffffffu, j_diag, 0);
       j_win = __shfl_sync(0xffffffffu, j_win, 0);
-      ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up) && wait(q_full + 8 * h, nq++ & 1, gave_up);
+      ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up, a.wait_clocks) && wait(q_full + 8 * h, nq++ & 1, gave_up, a.wait_clocks);
       if (!ok) break;
       tc_fence_after();
       scores();
       if (take > 1) {
-        ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up);
+        ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up, a.wait_clocks);
         if (!ok) break;
         scores();
       }
       for (int j = 0; j < take; ++j) {
         const bool more = j + 2 < take;
-        ok = wait(v_full + 8 * rv.stage, rv.phase, gave_up);
-        if (ok && more) ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up);
-        if (ok) ok = wait(p_full + 16 * h + 8 * (np & 1), np >> 1 & 1, gave_up);
+        ok = wait(v_full + 8 * rv.stage, rv.phase, gave_up, a.wait_clocks);
+        if (ok && more) ok = wait(k_full + 8 * rk.stage, rk.phase, gave_up, a.wait_clocks);
+        if (ok) ok = wait(p_full + 16 * h + 8 * (np & 1), np >> 1 & 1, gave_up, a.wait_clocks);
         if (!ok) break;
         tc_fence_after();
         int skip = 0;
@@ -348,22 +348,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (more) scores();
       }
     }
-    if (!ok) {  // products in flight end before tensor memory is freed
-      if (elect_one()) tc_commit(smem_u32(&sh.drain[h]));
-      __syncwarp();
-      for (int i = 0; i < 1 << 20 && !mbar_try(smem_u32(&sh.drain[h]), 0); ++i) {
-      }
-    }
+    // Products in flight end before tensor memory is freed.
+    if (elect_one()) tc_commit(smem_u32(&sh.drain[h]));
+    __syncwarp();
+    drain(smem_u32(&sh.drain[h]), 0);
   } else if (warp < kLoadWarp) {
     const int h = warp >> 2, wt = tid & 127, row = h * 128 + wt;  // half, thread of the warpgroup = row of the half
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + h * 2 * kBN, o_addr = tmem + lanes + o_col + h * D;
     const float c = a.scale_log2;
     uint32_t ns = 0, nm = 0, tiles = 0;  // S tiles, masked tiles of this half; tiles of the CTA
-    bool ok = true, q_in = false;
+    bool ok = a.wait_clocks > 0, q_in = false;
+    if (!ok) *gave_up = 1;
     // Waits for the products of tile ns - 1. (Two barriers in turn: the scores of tile ns - 1 came behind the products
     // of ns - 3, so that the phase waited for is the only one that can be open.)
-    auto pv_wait = [&] { return wait(pv_done + 16 * h + 8 * ((ns - 1) & 1), (ns - 1) >> 1 & 1, gave_up); };
+    auto pv_wait = [&] { return wait(pv_done + 16 * h + 8 * ((ns - 1) & 1), (ns - 1) >> 1 & 1, gave_up, a.wait_clocks); };
     // This half's query rows of an item into shared memory, asynchronously.
     auto load_q = [&](const Tile &item, int head) {
       const int n_rows = item.ntok * a.group;
@@ -409,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto tile = [&](int j, auto with_mask) -> bool {
         constexpr bool kMasked = decltype(with_mask)::value;
         const uint32_t buf = ns & 1, s_at = s_addr + buf * kBN;
-        if (!wait(s_full + 16 * h + 8 * buf, ns >> 1 & 1, gave_up)) return false;
+        if (!wait(s_full + 16 * h + 8 * buf, ns >> 1 & 1, gave_up, a.wait_clocks)) return false;
         tc_fence_after();
         if (j == w.take - 1) {  // the scores are done with Q: the next item's rows may come
           Walk next = w;
@@ -470,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
         if constexpr (kMasked) {
           const uint32_t nv = tiles + j;
-          if (!wait(v_full + 8 * (nv % S), (nv / S) & 1, gave_up)) return false;
+          if (!wait(v_full + 8 * (nv % S), (nv / S) & 1, gave_up, a.wait_clocks)) return false;
           unsigned char *vs = base_p + (v_base - base) + (nv % S) * KV::kTile;
           const int vr = wt >> 1, key = j * kBN + vr;  // two threads a V row
           bool bad = false;
@@ -489,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (bad) poison[nm % 3] = 1;
           if (wt == 0) poison[(nm + 1) % 3] = 0;
           mbar_arrive(v_seen + 8 * h);
-          if (!wait(v_seen + 8 * h, nm & 1, gave_up)) return false;
+          if (!wait(v_seen + 8 * h, nm & 1, gave_up, a.wait_clocks)) return false;
           const int poisoned = poison[nm++ % 3];
           if (wt == 0) *static_cast<volatile int *>(&sh.skip[h][buf]) = poisoned;
           if (poisoned) {
@@ -592,6 +591,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();  // O is read before the next item's products write it
     }
+    // After a wait that gave up, query rows and stores to tensor memory may be under way.
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    tc_wait_st();
   }
   tc_fence_before();
   __syncthreads();

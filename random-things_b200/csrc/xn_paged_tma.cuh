@@ -12,8 +12,6 @@ namespace xn {
 namespace paged {
 namespace {
 
-constexpr long long kWaitClocks = 4000000000ll;  // a wait gives up after 2 s or more
-
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
@@ -38,22 +36,29 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 }
 
 // Waits with a converged warp for the phase of `parity`; false when it did not
-// come within kWaitClocks or another role gave up (then nothing that the phase
-// stands for may be used). All lanes poll: with one lane polling in a branch of
+// come within `limit` clocks or another role gave up (then nothing that the
+// phase stands for may be used). All lanes poll: with one lane polling in a branch of
 // its own, what follows no longer counts as equal in all lanes, and operands
 // leave the uniform registers (measured: prefill of 8192 tokens 0.69 -> 0.89 ms).
-// Inlined: with a call in the kernel its register split would not take effect.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
+// The limit matters only behind the first look (tested before it: 589 -> 639 us).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *gave_up, long long limit) {
   bool got = mbar_try(bar, parity);
   if (!got) {
     const long long t0 = clock64();
     do {
 #pragma unroll 1
       for (int i = 0; i < 64 && !got; ++i) got = mbar_try(bar, parity);
-    } while (!got && !*gave_up && clock64() - t0 < kWaitClocks);
+    } while (!got && !*gave_up && clock64() - t0 < limit);
     if (!got) *gave_up = 1;
   }
   return __all_sync(0xffffffffu, got);
+}
+// The end of a role that copies or products in flight would outlive: waits for
+// the phase whoever gave up, and up to the full limit.
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try(bar, parity) && clock64() - t0 < kWaitClocks) {
+  }
 }
 // One arrival for a warp, behind what all its lanes did.
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
