@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             bad |= non_finite2<T>(x->x) | non_finite2<T>(x->y) | non_finite2<T>(x->z) | non_finite2<T>(x->w);
         }
         proxy_fence();  // before TMA writes the stage again
+        __syncwarp();   // other lanes read the zeroed rows (a vote orders no memory)
         poisoned = __any_sync(0xffffffffu, bad);
       }
       float top[2];

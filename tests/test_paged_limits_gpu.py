@@ -98,3 +98,18 @@ def test_attention_windows_longer_than_any_request(xn, cuda, dtype, new, window)
     want = b.run(xn)
     assert torch.equal(b.run(xn, window=window), want)
     b.check(xn, window=window)
+
+
+# -- attention: rows that no token sees ------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("window", [0, 1, 9])
+def test_attention_single_tokens_over_stale_rows(xn, cuda, dtype, d, window):
+    """Every count of unseen NaN rows in a key tile, at its end and before a window, in 64 requests at once, again and
+    again: the lanes that read the zeroed rows are others than those that zero them."""
+    b = Batch(cuda, dtype, 4, 2, d, 64, list(range(64)), [1] * 64, stale=float("nan"))
+    b.check(xn, window=window)
+    want = b.run(xn, window=window)
+    for _ in range(50):
+        assert torch.equal(b.run(xn, window=window), want)
