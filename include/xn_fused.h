@@ -452,8 +452,8 @@ XN_API int xn_paged_append_rope(void *q_out, void *k_pages, void *v_pages, const
  *
  * q rows start every q_tok_stride elements (a slice of a packed projection
  * will do). max_new is the largest t the caller expects: it chooses the kernel
- * (results hold for any t). scale is positive and finite; d is 32, 64 or 128;
- * h is a multiple of h_kv, h / h_kv <= 64; tensors are 16-byte aligned and
+ * (results hold for any t). scale is positive and at most 2^127; d is 32, 64 or
+ * 128; h is a multiple of h_kv, h / h_kv <= 64; tensors are 16-byte aligned and
  * strides multiples of 16 bytes. workspace (device, 16-byte aligned) holds at
  * least xn_paged_attention_workspace() bytes of these sizes; nothing in it
  * needs to be set, nothing is kept in it between calls, and calls that may run

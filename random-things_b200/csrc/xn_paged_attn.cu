@@ -442,7 +442,8 @@ int xn_paged_attention(void *out, const void *q, const void *k_pages, const void
   if (max_blocks < 0 || max_blocks > ((int64_t{1} << 31) - 1024) / page_size)
     return fail(XN_E_INVALID, "%s: max_blocks=%lld out of range", op, (long long)max_blocks);
   if (window < 0) return fail(XN_E_INVALID, "%s: negative window", op);
-  if (!(scale > 0.f) || isinf(scale)) return fail(XN_E_INVALID, "%s: scale must be positive and finite", op);
+  if (!(scale > 0.f) || scale > 0x1p127f)  // scale log2(e) is finite too
+    return fail(XN_E_INVALID, "%s: scale must be positive and at most 2^127", op);
   if (q_tok_stride < h * d || q_tok_stride % (16 / dtype_bytes(dtype)) != 0)
     return fail(XN_E_INVALID, "%s: q rows need a stride of at least h * d elements, a multiple of 16 bytes (got %lld)", op,
                 (long long)q_tok_stride);

@@ -206,12 +206,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float mc = m[r] == -INFINITY ? 0.f : -m[r] * c;
+        const float low = m[r] == -INFINITY ? 0.f : m[r];  // before the scale, as in the kernel for chunks
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 2 * r; j < 2 * r + 2; ++j) {
-            s[i][j] = ex2_approx_ftz(__fmaf_rn(s[i][j], c, mc));
+            s[i][j] = ex2_approx_ftz((s[i][j] - low) * c);
             l[r] += s[i][j];
           }
       }

@@ -2,7 +2,7 @@
 of these calls reaches a launch)."""
 import pytest
 
-from test_paged_cpu import _plan_args, _rc
+from test_paged_cpu import _attn_args, _plan_args, _rc
 
 # Arrays of 16 requests at addresses of their own, 4096 bytes apart.
 APART = dict(requests=16, token_cap=32, q_start=4096, kv_len=2 * 4096, positions=3 * 4096, slots=4 * 4096, ring_out=5 * 4096,
@@ -16,3 +16,13 @@ def test_plan_refuses_outputs_that_begin_or_end_inside_an_input(xn, kw):
     """One output shifted against an input by a few entries: other blocks would read what one has written."""
     assert _rc(xn, "xn_paged_plan", *_plan_args(**dict(APART, **kw))) == xn.XN_E_INVALID
     assert "input array" in xn.last_error()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127 * (1 + 2.0 ** -23), 2.5e38, 3.4e38])
+def test_attention_refuses_scales_past_f32_in_base_2(xn, scale):
+    assert _rc(xn, "xn_paged_attention", *_attn_args(scale=scale)) == xn.XN_E_INVALID
+    assert "scale" in xn.last_error()
+
+
+def test_attention_takes_the_largest_scale(xn):
+    assert _rc(xn, "xn_paged_attention", *_attn_args(scale=2.0 ** 127, n=0)) == xn.XN_OK

@@ -11,6 +11,8 @@ import pytest
 import torch
 
 import paged_ref
+from helpers import U32
+from paged_ref import HALF_STEP
 from test_paged_gpu import DT, Batch, _plan_state, _run_plan, i64
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +115,69 @@ def test_attention_single_tokens_over_stale_rows(xn, cuda, dtype, d, window):
     want = b.run(xn, window=window)
     for _ in range(50):
         assert torch.equal(b.run(xn, window=window), want)
+
+
+# -- attention: large scores -----------------------------------------------------
+
+def _one_key(dtype, value, h, hk, d, new, dev):
+    """Requests of one cached key each that every row sees alone or with copies of it: all of q and k is `value`."""
+    b = Batch(dev, dtype, h, hk, d, 16, [0] * 3, [1, new, 1])
+    b.q[:], b.k[:] = value, torch.where(torch.isnan(b.k), b.k, value)
+    return b
+
+
+# Scores of up to 128 x 60000^2 x scale (f16) and of 2^96 x scale (bf16, f32): finite in f32.
+HUGE = [("f16", 8000.0), ("f16", 60000.0), ("bf16", 8000.0), ("bf16", 60000.0), ("bf16", 2.0 ** 44), ("f32", 60000.0),
+        ("f32", 2.0 ** 44)]
+
+
+@pytest.mark.parametrize("dtype,value", HUGE)
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 64), (8, 1, 128), (2, 2, 32)])
+@pytest.mark.parametrize("new", [1, 90])
+@pytest.mark.parametrize("scale", [None, 1.0, 1e6, 2.0 ** 127])
+def test_attention_equal_scores_of_any_size(xn, cuda, dtype, value, h, hk, d, new, scale):
+    """Keys of one and the same score weigh alike, however large it is: rows of one key give its value, others the mean.
+
+    The scores of a row are sums of equal terms in equal order, so they are equal to the last bit and every weight is 1;
+    a chunk's bound is that of the weights' and the output's sums and rounding alone."""
+    b = _one_key(dtype, value, h, hk, d, new, cuda)
+    if scale is not None:
+        b.scale = scale
+    got = b.run(xn).view(-1, h, d).double().cpu()
+    for i, (lo, hi) in enumerate(zip(b.start, b.start[1:])):
+        v = b.v[b.table[i, :-(-b.kv[i] // 16)].long()].transpose(1, 2).reshape(-1, hk, d)[:b.kv[i]].double()
+        ref = torch.stack([v[:t + 1].mean(0) for t in range(hi - lo)]).repeat_interleave(h // hk, 1)
+        mag = torch.stack([v[:t + 1].abs().mean(0) for t in range(hi - lo)]).repeat_interleave(h // hk, 1)
+        # Up to 90 terms of weight 1 (exact in every type): 90 roundings of the sum, one of the quotient, one of the output.
+        tol = 92 * 2 * U32 * mag + HALF_STEP[DT[dtype]] * 1.01 * ref.abs()
+        assert ((got[lo:hi] - ref).abs() <= tol).all()
+        assert torch.equal(got[lo], v[0].repeat_interleave(h // hk, 0))  # one key: its value, exactly
+
+
+@pytest.mark.parametrize("dtype,value", HUGE)
+@pytest.mark.parametrize("new", [1, 90])
+@pytest.mark.parametrize("order", ["rising", "falling"])
+def test_attention_the_largest_of_huge_scores_takes_all(xn, cuda, dtype, value, new, order):
+    """Keys whose scores lie far apart: each row gives the value of its largest, whether the maximum moves with every
+    tile or stands from the first."""
+    h, hk, d, n = 4, 2, 64, 400
+    b = Batch(cuda, dtype, h, hk, d, 16, [n], [new])
+    kv = b.kv[0]
+    step = torch.linspace(0.25, 1.0, kv, dtype=torch.float64)
+    step = step if order == "rising" else step.flip(0)
+    at = b.table[0, :-(-kv // 16)].long()
+    rows = (value * step).to(DT[dtype])
+    keys = torch.zeros(at.numel() * 16, dtype=DT[dtype])
+    keys[:kv] = rows
+    b.k[at] = keys.view(-1, 1, 16, 1).expand(-1, hk, -1, d)
+    b.q[:] = value
+    got = b.run(xn).view(-1, h, d).double().cpu()
+    v = b.v[at].transpose(1, 2).reshape(-1, hk, d)[:kv].double()
+    exact = rows.double()
+    for t in range(new):
+        # Keys of the largest (rounded) size share the weight; the next smaller one is 2^-8 or more below, which is
+        # more than 2^20 in the exponent.
+        top = exact[:n + t + 1] == exact[:n + t + 1].max()
+        ref, mag = v[:n + t + 1][top].mean(0), v[:n + t + 1][top].abs().mean(0)
+        tol = (int(top.sum()) + 2) * 2 * U32 * mag + HALF_STEP[DT[dtype]] * 1.01 * ref.abs()
+        assert ((got[t] - ref.repeat_interleave(h // hk, 0)).abs() <= tol.repeat_interleave(h // hk, 0)).all(), t
