@@ -370,7 +370,10 @@ class PagedStreamingDecoder:
     fused LayerNorm, MLP. Rows behind the last frame are padding: what comes out
     there means nothing. Nothing waits for the host, so that a captured graph
     can hold the step; err_flag (int32) tells of steps that did not fit, which
-    change nothing."""
+    change nothing: those that need more pages or frames than there are, and
+    those that would take a stream past max_len positions (by default
+    cfg.max_seq_len; at most the rows of cos and sin). A stream holds its pages
+    until it ends, those before its last `context` positions too."""
 
     def __init__(self, cfg: MimiChainConfig, weights: dict[str, torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
                  streams: int, pages: int, token_cap: int, *, max_new: int | None = None, page_size: int = 16,
@@ -386,7 +389,10 @@ class PagedStreamingDecoder:
         self.scale = 1.0 / math.sqrt(hd)
         self.k = [torch.zeros((pages, H, page_size, hd), dtype=dtype, device=dev) for _ in range(cfg.num_layers)]
         self.v = [torch.zeros_like(k) for k in self.k]
-        blocks = -(-(cfg.max_seq_len if max_len is None else max_len) // page_size)
+        self.max_len = cfg.max_seq_len if max_len is None else int(max_len)
+        if not 0 < self.max_len <= cos.shape[0]:
+            raise ValueError(f"max_len {self.max_len} is not within the {cos.shape[0]} rows of the rotation tables")
+        blocks = -(-self.max_len // page_size)
         self.table = torch.full((streams, blocks), -1, dtype=torch.int32, device=dev)
         self.ring = torch.arange(pages, dtype=torch.int32, device=dev)
         self.ring_state = torch.tensor([0, pages], dtype=torch.int64, device=dev)
@@ -396,6 +402,10 @@ class PagedStreamingDecoder:
 
     def step(self, x: torch.Tensor, new: torch.Tensor) -> torch.Tensor:
         cfg, w, eps, H = self.cfg, self.w, self.cfg.eps, self.cfg.num_heads
+        if self.max_len < self.table.shape[1] * self.page_size:
+            # The last page goes on behind max_len, which the plan does not know: a step that would use that asks for
+            # more tokens than fit.
+            new = torch.where((self.lens + new > self.max_len).any(), self.token_cap + 1, new)
         plan = xn.paged_plan(self.lens, new, self.table, self.ring, self.ring_state, self.page_size, self.token_cap,
                              err_flag=self.err_flag)
         resid = x
