@@ -42,8 +42,11 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
   return r;
 }
 
-// mag / 448, correctly rounded for normal results: one FMA step on the product
-// with the rounded reciprocal (an infinite mag has no remainder).
+// mag / 448, correctly rounded: Markstein's correction of a quotient, one FMA
+// step on the product with the rounded reciprocal (an infinite mag has no
+// remainder). Half ways between subnormal results may go to either side: there
+// the remainder's product with a rounded reciprocal decides. (The division
+// itself, for all or for subnormal results alone: 32768 x 4096 by groups 3% slower.)
 __device__ __forceinline__ float scale_of(float mag) {
   constexpr float r = 1.f / 448.f;
   const float q = __fmul_rn(mag, r);

@@ -181,3 +181,29 @@ def test_attention_the_largest_of_huge_scores_takes_all(xn, cuda, dtype, value, 
         ref, mag = v[:n + t + 1][top].mean(0), v[:n + t + 1][top].abs().mean(0)
         tol = (int(top.sum()) + 2) * 2 * U32 * mag + HALF_STEP[DT[dtype]] * 1.01 * ref.abs()
         assert ((got[t] - ref.repeat_interleave(h // hk, 0)).abs() <= tol.repeat_interleave(h // hk, 0)).all(), t
+
+
+# -- 8-bit norm ------------------------------------------------------------------
+
+def test_norm_q8_scale_is_the_quotient_by_448(xn, cuda):
+    """Rows of ones under an eps that vanishes have y = alpha exactly: each group's scale is alpha / 448, rounded once,
+    from the smallest magnitude to the largest and infinity."""
+    g = torch.Generator().manual_seed(1)
+    bits = torch.randint(1, 0x7f800000, (1 << 16,), generator=g)
+    small = torch.randint(1, 0x05000000, (1 << 14,), generator=g)  # subnormal quotients, and the first normal ones
+    edges = [1, 2, 223, 224, 225, 448, 0x7fffff, 0x800000, 0x800001, 0x7f7fffff, 0x7f800000]
+    edges += [(e << 23) + m for e in range(1, 255) for m in (0, 1, 0x600000, 0x5fffff, 0x600001, 0x7fffff)]
+    mag = torch.cat([bits, small, torch.tensor(edges)]).int().view(torch.float32)
+    # A quotient of 24 bits by 7 is never as near to half way between two normal floats as the double's rounding.
+    want = (mag.double() / 448.0).float()
+    normal = want >= 2.0 ** -126
+    assert normal.sum() > 60000 and (~normal).sum() > 10000
+    alpha = mag.repeat_interleave(32).to(cuda)
+    x = torch.ones(1, alpha.numel(), device=cuda)
+    for lo, n in ((0, 8192), (1 << 21, 8192), (0, alpha.numel())):  # rows in registers, a row too wide for them
+        _, s, _ = xn.rms_norm_q8(x[:, lo:lo + n], alpha[lo:lo + n], 1e-30, group=32)
+        s, part = s[0].cpu(), slice(lo // 32, (lo + n) // 32)
+        assert torch.equal(torch.where(normal[part], s, 0.0), torch.where(normal[part], want[part], 0.0))
+        # Subnormal: half a step of 2^-149, either way of a half, and the step's own 2^-24 of a step.
+        off = (s.double() - mag[part].double() / 448.0).abs()[~normal[part]]
+        assert (off <= 2.0 ** -150 * (1 + 2.0 ** -23)).all()
