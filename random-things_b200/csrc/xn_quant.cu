@@ -352,7 +352,9 @@ int launch_q8(const Q8Params &p, cudaStream_t st, const char *op) {
   };
   constexpr int V = Elem<T>::kVec;
   bool done = false;
-  if (fits(V))
+  if (p.cols == 0)  // scales alone, all 0: the kernel for wide rows has nothing else to do
+    ;
+  else if (fits(V))
     done = p.group != 0 ? launch_q8_rows<T, V, true>(p, st) : launch_q8_rows<T, V, false>(p, st);
   else if (p.group == 0)
     done = fits(2) ? launch_q8_rows<T, 2, false>(p, st) : launch_q8_rows<T, 1, false>(p, st);
@@ -375,9 +377,9 @@ extern "C" int xn_rms_norm_q8(void *dst, float *scales, void *residual_out, cons
     return fail(XN_E_INVALID, "%s: group %lld not in {0, 32, 64, 128}", op, (long long)group);
   if (group != 0 && cols % group != 0)
     return fail(XN_E_INVALID, "%s: group %lld does not divide cols=%lld", op, (long long)group, (long long)cols);
-  if (rows == 0 || cols == 0) return ok();
+  if (rows == 0 || (cols == 0 && group != 0)) return ok();
   if (rows > 0x7fffffffLL) return fail(XN_E_INVALID, "%s: too many rows (%lld)", op, (long long)rows);
-  if (dst == nullptr || scales == nullptr || src == nullptr || alpha == nullptr)
+  if (scales == nullptr || (cols > 0 && (dst == nullptr || src == nullptr || alpha == nullptr)))
     return fail(XN_E_INVALID, "%s: null pointer", op);
   Q8Params p{static_cast<uint8_t *>(dst), scales, residual_out, src, alpha, branch, rows, cols, 0,
              static_cast<int>(group), eps};

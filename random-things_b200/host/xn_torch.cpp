@@ -330,7 +330,9 @@ PyObject *rms_norm_q8(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int64_t group = integer(a[4]);
     at::Tensor out = maybe(a[5], op, "out"), scales = maybe(a[6], op, "scales"), res = maybe(a[7], op, "residual_out");
     if (!(eps > 0.0)) refuse(XN_E_INVALID, op, " eps must be positive");
-    const int64_t cols = x.dim() > 0 ? x.size(-1) : 1, rows = cols > 0 ? x.numel() / cols : 0;
+    const int64_t cols = x.dim() > 0 ? x.size(-1) : 1;
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
     if ((group != 0 && group != 32 && group != 64 && group != 128) || (group != 0 && cols % group != 0))
       refuse(XN_E_INVALID, op, ": group ", group, " is not 0, 32, 64 or 128 and a divisor of ", cols);
     has_shape(op, "alpha", alpha, {cols});

@@ -2,7 +2,7 @@
 of these calls reaches a launch)."""
 import pytest
 
-from test_paged_cpu import _attn_args, _plan_args, _rc
+from test_paged_cpu import BF16, _attn_args, _plan_args, _rc
 
 # Arrays of 16 requests at addresses of their own, 4096 bytes apart.
 APART = dict(requests=16, token_cap=32, q_start=4096, kv_len=2 * 4096, positions=3 * 4096, slots=4 * 4096, ring_out=5 * 4096,
@@ -26,3 +26,10 @@ def test_attention_refuses_scales_past_f32_in_base_2(xn, scale):
 
 def test_attention_takes_the_largest_scale(xn):
     assert _rc(xn, "xn_paged_attention", *_attn_args(scale=2.0 ** 127, n=0)) == xn.XN_OK
+
+
+def test_norm_of_no_columns_still_has_scales(xn):
+    """Rows of no columns have a scale each: the call needs a place for them, and nothing else."""
+    norm = lambda scales, group: _rc(xn, "xn_rms_norm_q8", None, scales, None, None, None, None, 5, 0, group, 1e-5, BF16, None)  # noqa: E731
+    assert norm(None, 0) == xn.XN_E_INVALID and "null" in xn.last_error()
+    assert norm(None, 32) == xn.XN_OK

@@ -207,3 +207,10 @@ def test_norm_q8_scale_is_the_quotient_by_448(xn, cuda):
         # Subnormal: half a step of 2^-149, either way of a half, and the step's own 2^-24 of a step.
         off = (s.double() - mag[part].double() / 448.0).abs()[~normal[part]]
         assert (off <= 2.0 ** -150 * (1 + 2.0 ** -23)).all()
+
+
+def test_norm_q8_rows_of_no_columns(xn, cuda):
+    """The largest of no values is 0, and so is the scale."""
+    s = torch.full((5,), 7.0, device=cuda)
+    q, got, _ = xn.rms_norm_q8(torch.empty(5, 0, device=cuda), torch.empty(0, device=cuda), 1e-5, scales=s)
+    assert got is s and s.eq(0).all() and q.shape == (5, 0)
