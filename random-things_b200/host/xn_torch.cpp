@@ -10,8 +10,10 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <exception>
 #include <sstream>
 #include <string>
 
@@ -142,7 +144,8 @@ at::Tensor part(const at::Tensor &buf, int64_t at, int64_t n) {
 
 PyObject *wrap(const at::Tensor &t) { return THPVariable_Wrap(t); }
 
-// Runs f, turning what it throws into a Python exception.
+// Runs f, turning what it throws into a Python exception: torch's own (an
+// allocation that fails, for one) into those that torch's operators raise.
 template <typename F>
 PyObject *guarded(F f) {
   try {
@@ -153,8 +156,8 @@ PyObject *guarded(F f) {
       Py_DECREF(x);
     }
   } catch (const PyFailed &) {
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }

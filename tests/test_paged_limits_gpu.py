@@ -214,3 +214,18 @@ def test_norm_q8_rows_of_no_columns(xn, cuda):
     s = torch.full((5,), 7.0, device=cuda)
     q, got, _ = xn.rms_norm_q8(torch.empty(5, 0, device=cuda), torch.empty(0, device=cuda), 1e-5, scales=s)
     assert got is s and s.eq(0).all() and q.shape == (5, 0)
+
+
+# -- binding ---------------------------------------------------------------------
+
+def test_out_of_memory_is_torchs_exception(xn, cuda):
+    """An output that cannot be allocated raises what torch's own operators raise, and nothing is lost."""
+    ring = torch.arange(8, dtype=torch.int32, device=cuda)
+    args = i64([0], cuda), i64([1], cuda), torch.full((1, 1), -1, dtype=torch.int32, device=cuda), ring, i64([0, 8], cuda), 8
+    torch.cuda.set_per_process_memory_fraction(0.05)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            xn.paged_plan(*args, (1 << 31) - 1)  # 34 GB
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert xn.paged_plan(*args, 1).slots.tolist() == [0]
