@@ -61,6 +61,11 @@ int64_t integer(PyObject *o) {
   if (v == -1 && PyErr_Occurred()) throw PyFailed{};
   return v;
 }
+bool truth(PyObject *o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PyFailed{};
+  return v != 0;
+}
 double real(PyObject *o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw PyFailed{};
@@ -232,7 +237,7 @@ PyObject *paged_append_rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const at::Tensor &k = tensor(a[5], op, "k_pages"), &v = tensor(a[6], op, "v_pages");
     const at::Tensor &pos = tensor(a[7], op, "positions"), &slots = tensor(a[8], op, "slots");
     const int64_t h = integer(a[1]), hk = integer(a[2]);
-    const int interleaved = PyObject_IsTrue(a[9]);
+    const bool interleaved = truth(a[9]);
     const at::Tensor err = maybe(a[10], op, "err_flag");
     at::Tensor q = maybe(a[11], op, "q_out");
     const Pool c = pool(op, k, v);

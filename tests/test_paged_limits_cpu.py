@@ -1,6 +1,7 @@
 """Refusals of the paged-cache operators at the ends of what they accept (none
 of these calls reaches a launch)."""
 import pytest
+import torch
 
 from test_paged_cpu import BF16, _attn_args, _plan_args, _rc
 
@@ -33,3 +34,18 @@ def test_norm_of_no_columns_still_has_scales(xn):
     norm = lambda scales, group: _rc(xn, "xn_rms_norm_q8", None, scales, None, None, None, None, 5, 0, group, 1e-5, BF16, None)  # noqa: E731
     assert norm(None, 0) == xn.XN_E_INVALID and "null" in xn.last_error()
     assert norm(None, 32) == xn.XN_OK
+
+
+class NoTruth:
+    def __bool__(self):
+        raise ValueError("no truth value")
+
+
+def test_what_an_argument_raises_comes_through(xn):
+    """An argument whose truth value raises stops the call with that, before anything else is looked at."""
+    pool = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    i = torch.zeros(4, dtype=torch.int64)
+    table = torch.zeros(9, 32, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="no truth value"):
+        xn.paged_append_rope(torch.zeros(4, 12 * 64, dtype=torch.bfloat16), 8, 2, table, table, pool, pool, i, i,
+                             interleaved=NoTruth())
