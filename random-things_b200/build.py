@@ -6,7 +6,8 @@ Usage: python random-things_b200/build.py [--force] [--verbose]
 Each csrc/*.cu file is compiled to an object with nvcc for sm_100a only, then
 linked into one shared library next to this file. The C ABI it exports is
 declared in include/xn_fused.h. Objects are rebuilt when their source or any
-header is newer.
+header is newer. The binding needs torch and Python's headers; without them the
+command builds the library alone, which is all that C, C++ and Rust callers use.
 """
 from __future__ import annotations
 
@@ -98,6 +99,18 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     return LIB_PATH
 
 
+def binding_lacks() -> str | None:
+    """What the binding cannot be built without here, or None."""
+    import importlib.util
+    import sysconfig
+
+    if importlib.util.find_spec("torch") is None:
+        return "torch is not installed"
+    if not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        return "Python's headers are not installed"
+    return None
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> Path:
     """host/xn_torch.cpp against this Python's torch, linked with libxn_fused.so
     next to it."""
@@ -131,7 +144,11 @@ def main(argv: list[str] | None = None) -> int:
     a = ap.parse_args(argv)
     path = build(force=a.force, verbose=a.verbose, ptxas_verbose=a.ptxas_verbose)
     print(path)
-    print(build_binding(force=a.force, verbose=a.verbose))
+    lacks = binding_lacks()
+    if lacks is None:
+        print(build_binding(force=a.force, verbose=a.verbose))
+    else:
+        print(f"{BINDING_PATH.name}, the Python binding, is not built: {lacks}", file=sys.stderr)
     return 0
 
 
