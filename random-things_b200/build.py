@@ -113,14 +113,19 @@ def binding_lacks() -> str | None:
 
 def build_binding(force: bool = False, verbose: bool = False) -> Path:
     """host/xn_torch.cpp against this Python's torch, linked with libxn_fused.so
-    next to it."""
+    next to it. Built again when a source is newer or the torch or Python that
+    it was built against is another one."""
     import sysconfig
 
+    import torch
     from torch.utils import cpp_extension
 
+    built_for = "\n".join([sys.version, str(sysconfig.get_config_var("SOABI")), torch.__version__, str(torch.__file__)])
+    stamp = BUILD_DIR / (BINDING_PATH.stem + ".built_for")
     src = PKG_DIR / "host" / "xn_torch.cpp"
     newest = max(src.stat().st_mtime, (INCLUDE / "xn_fused.h").stat().st_mtime, LIB_PATH.stat().st_mtime)
-    if not force and BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= newest:
+    same = stamp.exists() and stamp.read_text() == built_for
+    if not force and same and BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= newest:
         return BINDING_PATH
     cxx = host_compiler()[1:] or ["g++"]
     inc = [f"-I{p}" for p in (INCLUDE, sysconfig.get_paths()["include"], *cpp_extension.include_paths(device_type="cuda"))]
@@ -133,6 +138,8 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING_PATH)
+    BUILD_DIR.mkdir(exist_ok=True)
+    stamp.write_text(built_for)
     return BINDING_PATH
 
 

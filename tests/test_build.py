@@ -1,10 +1,21 @@
 """The build's second part, the Python binding: left out where torch is not
-there."""
+there, built again for another torch or Python."""
+import importlib.util
 import subprocess
 import sys
 from pathlib import Path
 
+import pytest
+
 BUILD = Path(__file__).resolve().parents[1] / "random-things_b200" / "build.py"
+
+
+@pytest.fixture
+def build():
+    spec = importlib.util.spec_from_file_location("xn_build", BUILD)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
 
 
 def test_the_library_alone_without_torch():
@@ -24,3 +35,33 @@ def test_the_library_alone_without_torch():
     assert out.returncode == 0, out.stderr
     assert "libxn_fused.so" in out.stdout and "xn_torch.so" not in out.stdout
     assert "xn_torch.so" in out.stderr and "torch is not installed" in out.stderr
+
+
+def test_the_binding_is_built_again_for_another_torch(build, monkeypatch, tmp_path):
+    runs = []
+
+    def run(cmd, check):
+        runs.append(cmd)
+        Path(cmd[cmd.index("-o") + 1]).write_text("built")
+
+    lib = tmp_path / "libxn_fused.so"
+    lib.write_text("")
+    monkeypatch.setattr(build, "LIB_PATH", lib)
+    monkeypatch.setattr(build, "BINDING_PATH", tmp_path / "xn_torch.so")
+    monkeypatch.setattr(build, "BUILD_DIR", tmp_path / "_build")
+    monkeypatch.setattr(build.subprocess, "run", run)
+    import torch
+
+    build.build_binding()
+    build.build_binding()
+    assert len(runs) == 1
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + ".other")
+    build.build_binding()
+    build.build_binding()
+    assert len(runs) == 2
+    monkeypatch.setattr(build.sys, "version", "another Python")
+    build.build_binding()
+    build.build_binding()
+    assert len(runs) == 3
+    build.build_binding(force=True)
+    assert len(runs) == 4
