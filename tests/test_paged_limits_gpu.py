@@ -183,6 +183,22 @@ def test_attention_the_largest_of_huge_scores_takes_all(xn, cuda, dtype, value, 
         assert ((got[t] - ref.repeat_interleave(h // hk, 0)).abs() <= tol.repeat_interleave(h // hk, 0)).all(), t
 
 
+# -- attention: groups and hints -------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("h,hk,d", [(21, 1, 64), (33, 1, 32), (64, 1, 128), (48, 2, 64), (128, 2, 32)])
+def test_attention_wide_groups(xn, cuda, dtype, h, hk, d):
+    Batch(cuda, dtype, h, hk, d, 16, [300, 5, 0], [1, 1, 1]).check(xn)
+    Batch(cuda, dtype, h, hk, d, 32, [200, 0, 70], [30, 17, 1], packed=True).check(xn, window=40)
+
+
+@pytest.mark.parametrize("hint", [0, 1, 4, 100])
+def test_attention_hint_f16(xn, cuda, hint):
+    Batch(cuda, "f16", 8, 2, 128, 16, [100, 1000, 5], [1, 1, 1]).check(xn, max_new=hint)
+    Batch(cuda, "f16", 8, 2, 64, 16, [100, 1000, 5], [50, 7, 30]).check(xn, max_new=hint)
+
+
+
 # -- 8-bit norm ------------------------------------------------------------------
 
 def test_norm_q8_scale_is_the_quotient_by_448(xn, cuda):
