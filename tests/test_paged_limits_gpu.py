@@ -199,6 +199,45 @@ def test_attention_hint_f16(xn, cuda, hint):
 
 
 
+# -- attention: the largest sizes --------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("hint", [1, 64])
+def test_attention_as_many_requests_as_there_may_be(xn, cuda, dtype, hint):
+    g = torch.Generator().manual_seed(1)
+    lens = torch.randint(0, 12, (xn.XN_PAGED_MAX_REQUESTS,), generator=g).tolist()
+    Batch(cuda, dtype, 2, 1, 32, 8, lens, [1] * len(lens)).check(xn, max_new=hint)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("window", [1, 100, 1000])
+def test_attention_positions_up_to_the_last(xn, cuda, dtype, new, window):
+    """A window at the end of the longest request there may be, its pages three that repeat."""
+    page, h, hk, d, dt = 256, 4, 2, 64, DT[dtype]
+    blocks = (2 ** 31 - 1024) // page
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(3, hk, page, d, generator=g).to(dt) for _ in range(2))
+    q = torch.randn(new, h, d, generator=g).to(dt)
+    table = (torch.arange(blocks, dtype=torch.int32) % 3).view(1, -1)
+    kv, start, scale = blocks * page, i64([0, new]), d ** -0.5
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    got = xn.paged_attention(q.to(cuda), k.to(cuda), v.to(cuda), table.to(cuda), start.to(cuda), i64([kv], cuda), scale,
+                             max_new=new, window=window, err_flag=err)
+    # The same request without the blocks that no token sees.
+    first = (kv - new - window) // page
+    ref, tol = paged_ref.attention(q, k, v, table[:, first:], start, i64([kv - first * page]), scale, window)
+    paged_ref.check_attention(got, ref, tol)
+    assert int(err) == 0
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("new", [1, 20])
+def test_attention_long_history(xn, cuda, dtype, new):
+    """A third of a million keys of one head: every part of the work list a piece of the same few rows."""
+    Batch(cuda, dtype, 4, 1, 64, 256, [333333], [new]).check(xn)
+
+
 # -- 8-bit norm ------------------------------------------------------------------
 
 def test_norm_q8_scale_is_the_quotient_by_448(xn, cuda):
