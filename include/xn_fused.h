@@ -482,7 +482,9 @@ XN_API int xn_paged_attention_workspace(int64_t *bytes, int64_t n_tokens, int64_
  *   h = src, or T(src + branch); residual_out = h if not NULL
  *   y = h / sqrt(sum(h^2)/cols + eps) * alpha[col]             (f32)
  *   scales[row, g] = max |y| over the g-th `group` columns / 448
- *   dst = e4m3(y / scale), 0 where the scale is 0 (as for a row of no columns)
+ *   dst = e4m3(y * (1 / scale)), 0 where the scale is 0 (as for a row of no
+ *         columns); the reciprocal is rounded to f32, so that a y / scale next
+ *         to half way between two e4m3 values may become either
  * so that dst * scale stands for y. group is 0 (one scale per row, scales
  * [rows]) or 32, 64 or 128 and a divisor of cols (scales [rows, cols/group]).
  * dst holds OCP e4m3 bytes (448 the largest value). A NaN among a group's y

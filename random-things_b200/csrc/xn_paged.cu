@@ -192,8 +192,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
 // written once. A work item is two 16-byte vectors: one of each half of a head
 // row (half-split) or two neighbouring ones (interleaved). A thread reads its
 // item before it knows the token's slot and position, which the tables wait
-// for: 129 us for 32768 tokens of 48 heads of 128, 95% of the measured copy
-// rate (slot first: 154 us; two items a thread: 135 us).
+// for (timed against each other: this order 129, slot first 154, two items a
+// thread 135 us). 32768 tokens of 48 heads of 128 now take 143 to 147 us, 0.85
+// of the measured copy rate.
 // ---------------------------------------------------------------------------
 struct PagedAppendParams {
   void *q_out, *k_pages, *v_pages;

@@ -10,9 +10,10 @@
 // The scores of the next two tiles are issued ahead, so that a half's softmax
 // need not wait for its own products. (With one buffer of 128 keys each half
 // went softmax, products, softmax, ...: an 8192-token prompt of 32 / 8 heads of
-// 128 took 632 us against 547; now 514, 0.66 of the measured bf16 rate. With
-// keys by 64 the score products read shared memory as fast as it goes, which
-// bounds the kernel together with the exponentials.) One more warp loads: K and V tiles come by TMA, a box
+// 128 took 632 us against 547. Now it takes 522 us alone and up to 581 in calls
+// back to back, as the power limit lets the clock go: 0.65 to 0.58 of the
+// measured bf16 rate. With keys by 64 the score products read shared memory as
+// fast as it goes, which bounds the kernel together with the exponentials.) One more warp loads: K and V tiles come by TMA, a box
 // per page, swizzled as the MMA reads them, through two rings of stages.
 //
 // O stays in tensor memory for all key tiles. When a row's maximum grows by
@@ -134,8 +135,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // 2^x on the FMA pipe, for a quarter of the weights: the exponential unit's 16
-// results a clock an SM take as long as the products (an 8192-token prompt 538
-// us without, 514 us with it; ragged f16 chunks 221 and 229 us).
+// results a clock an SM take as long as the products. An 8192-token prompt of 32
+// / 8 heads without and with it, alone: of 128 553 and 514 us (f16 555 and 521),
+// of 64 493 and 469 (f16 496 and 469), of 32 471 and 457 (f16 471 and 451);
+// ragged chunks of 12 requests, 24 / 8 heads: of 128 242 and 242 us (f16 244 and
+// 242), of 64 203 and 197 (f16 205 and 197), of 32 191 and 186 (f16 191 and 184).
 // x = n + f, |f| <= 1/2: adding 1.5 2^23 + 127 leaves n + 127 in the low bits,
 // which shifted into place are 2^n; 2^f is a minimax polynomial (fit_exp2.py,
 // relative error 2.7e-6, against 2^-9 or 2^-12 for the rounding that follows).

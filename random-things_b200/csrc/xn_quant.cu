@@ -2,14 +2,14 @@
 // (OCP e4m3) with one f32 scale per row or per group of columns, for sm_100a.
 //
 //   h = src or T(src + branch); y = h * (1 / sqrt(sum h^2 / cols + eps)) * alpha
-//   scale = max |y| / 448;  dst = e4m3(y * (1 / scale))
+//   scale = max |y| / 448;  dst = e4m3(y * (1 / scale)), the reciprocal rounded
 //
 // Bytes bound: src, branch and h cross memory once in T, dst in one byte. The
 // row stays in registers between the sum of squares, the largest magnitude and
 // the conversion. All of it is f32; the roundings are h (the residual stream's
 // own type), y's f32 operations, and the one to e4m3. Measured: 32768 x 4096
-// bf16 with a residual 141 us (one scale a row) and 163 us (groups of 128),
-// 1.0 and 0.88 of the measured copy rate.
+// bf16 with a residual 143 us (one scale a row) and 163 to 179 us (groups of
+// 128), 1.0 and 0.80 to 0.88 of the measured copy rate.
 #include <cuda_fp8.h>
 
 #include <type_traits>
